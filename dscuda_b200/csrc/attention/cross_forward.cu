@@ -1,0 +1,542 @@
+// Cross attention forward (D = 128, grouped-query) on tcgen05: the queries of a decoder over an encoder's states, each entry with its own
+// number of valid keys, no causal mask.
+//
+// Rows.  All query heads of a key head see the same keys, so their queries are the rows of one matrix, row = token * group + head: a TMA box
+// of {64 columns, group heads, tokens} lays them out that way (a group that does not divide 128 leaves the last rows of a tile
+// unused).  Short queries fill their tiles and a key tile is fetched once for a whole group.
+//
+// A CTA takes two 128-row tiles of one (entry, key head), which alternate on the tensor core: S = Q K^T into tensor memory, online softmax
+// with one thread to a row, P back into tensor memory as bf16 (P aliases S) and O += P V.  K and V stream through a ring of 16 KB chunks.  Warps
+// 0-3 and 4-7 are the softmax of the two tiles, warp 8 issues the MMAs, warp 9 the loads; warps 10 and 11 clear the value rows behind an
+// entry's length (a weight of zero does not keep their NaN out of P V) and complete the third warpgroup, which hands registers to the
+// softmax.  The schedule is that of prefill_forward.cu, where its measurements stand.
+//
+// Few rows to a key head (single tokens) go to flash_decode.cu instead, which splits the keys over the SMs.
+//
+// P is rounded to bf16 (half a step is 2^-9 of each weight); sums, maxima and O are fp32.  Every wait is bounded.
+#include "flash_attention.h"
+#include "cuda_common.h"
+#include "attention_internal.h"
+#include "sm100_primitives.cuh"
+#include "../common/launch.h"
+#include "../common/tensor_map.h"
+
+#include <stdexcept>
+
+namespace dscuda {
+namespace {
+
+using namespace sm100;
+
+constexpr int HEAD = 128;
+constexpr int TILE = 128;                   // rows of a query tile, keys of a key tile
+constexpr int CHUNK = 128 * 128;            // 16 KB: 128 rows x 64 bf16, or 64 keys x 128
+constexpr int RING = 10;
+constexpr int PER_TILE = 4;                 // ring chunks of a key tile: two of K, two of V
+constexpr int Q_BYTES = 4 * CHUNK;
+constexpr int MISC_BYTES = 1024;
+constexpr int SMEM_BYTES = Q_BYTES + RING * CHUNK + MISC_BYTES + 1024;
+constexpr int THREADS = 384;
+constexpr int MMA_WARP = 8;
+constexpr int LOAD_WARP = 9;
+constexpr int TAIL_WARP = 10;
+constexpr int TMEM_COLUMNS = 512;           // S0 | S1 | O0 | O1
+constexpr float RESCALE_THRESHOLD = 8.0F;   // log2 units; below it the old row maximum is kept
+constexpr float LOG2E = 1.4426950408889634F;
+
+__device__ int cross_forward_status = 0;
+
+struct CrossForwardParams {
+    CUtensorMap q;              // group rows, box {64, group, tokens of a tile}
+    CUtensorMap k;              // [B][Tk][Hkv * 128], boxes of 128 rows
+    CUtensorMap v;              // boxes of 64 rows
+    CUtensorMap out;            // like q
+    float* lse;                 // [B, Hq, Tq]
+    const int* lengths;         // null: Tk
+    int tokens, keys, heads, group;
+    int tile_tokens;            // tokens of a query tile
+    float scale, scale_log2;
+};
+
+struct Barriers {
+    uint64_t q_full[2];
+    uint64_t s_full[2];
+    uint64_t p_full[2];
+    uint64_t p_half[2];
+    uint64_t staged[2];         // the tile's output rows are in shared memory
+    uint64_t ring_full[RING];
+    uint64_t ring_empty[RING];
+    uint64_t tail_full[2];
+    uint32_t tmem_base;
+    int abort_flag;
+};
+static_assert(sizeof(Barriers) <= MISC_BYTES, "barrier block too large");
+
+__global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_constant__ CrossForwardParams p) {
+    extern __shared__ uint8_t smem_raw[];
+    if (*reinterpret_cast<volatile int*>(&cross_forward_status) != 0) {
+        grid_dependency_wait();
+        return;
+    }
+    const int entry = blockIdx.z;
+    const int kv_head = blockIdx.y;
+    const int row_tiles = (p.tokens + p.tile_tokens - 1) / p.tile_tokens;
+    const int tile0 = blockIdx.x * 2;
+    const bool second = tile0 + 1 < row_tiles;
+
+    const uint32_t smem_base = (smem_u32(smem_raw) + 1023U) & ~1023U;
+    uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
+    const uint32_t ring_smem = smem_base + Q_BYTES;
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + Q_BYTES + RING * CHUNK);
+    volatile int* abort_flag = &bars->abort_flag;
+    const int warp = threadIdx.x / 32;
+    const int lane = threadIdx.x % 32;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(smem_u32(&bars->q_full[i]), 1);
+            mbar_init(smem_u32(&bars->s_full[i]), 1);
+            mbar_init(smem_u32(&bars->p_full[i]), TILE);
+            mbar_init(smem_u32(&bars->p_half[i]), TILE);
+            mbar_init(smem_u32(&bars->staged[i]), TILE);
+            mbar_init(smem_u32(&bars->tail_full[i]), 1);
+        }
+        for (int i = 0; i < RING; ++i) {
+            mbar_init(smem_u32(&bars->ring_full[i]), 1);
+            mbar_init(smem_u32(&bars->ring_empty[i]), 1);
+        }
+        bars->abort_flag = 0;
+        mbar_init_fence();
+    }
+    if (warp == MMA_WARP) {
+        tmem_alloc(smem_u32(&bars->tmem_base), TMEM_COLUMNS);
+        tmem_relinquish();
+    }
+    if (warp == LOAD_WARP && lane == 0) {
+        tma_prefetch_descriptor(&p.q);
+        tma_prefetch_descriptor(&p.k);
+        tma_prefetch_descriptor(&p.v);
+    }
+    tc_fence_before_sync();
+    __syncthreads();
+    tc_fence_after_sync();
+    grid_dependency_wait();
+    const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
+    const int length = p.lengths == nullptr ? p.keys : min(max(p.lengths[entry], 0), p.keys);
+    const int tile_count = (length + TILE - 1) / TILE;
+    // what lies between the length and the end of the entry's states may be anything; behind that end the loads give zeros
+    const int tail_keys = length < p.keys ? length - (tile_count - 1) * TILE : TILE;
+
+    constexpr int REG_LO = 88;
+    constexpr int REG_HI = 208;
+    static_assert(8 * (REG_HI - 168) <= 4 * (168 - REG_LO), "register redistribution exceeds the CTA's allocation");
+    if (warp >= 8) {
+        reg_dealloc<REG_LO>();
+        if (warp >= TAIL_WARP) {
+            if (tail_keys < TILE && tile_count > 0) {
+                const int half = warp - TAIL_WARP;
+                if (__all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->tail_full[half]), 0, abort_flag, &cross_forward_status))) {
+                    const int slot = ((tile_count - 1) * PER_TILE + 2 + half) % RING;
+                    uint8_t* chunk = smem + Q_BYTES + slot * CHUNK;
+                    const int first = min(max(tail_keys - half * 64, 0), 64);
+                    clear_rows(chunk, first, 64, lane);
+                    clear_rows(chunk + CHUNK / 2, first, 64, lane);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(smem_u32(&bars->ring_full[slot]));
+                    }
+                }
+            }
+        } else if (warp == LOAD_WARP) {
+            if (lane == 0 && tile_count > 0) {
+                auto load_q = [&](int i) {
+                    const uint32_t bar = smem_u32(&bars->q_full[i]);
+                    mbar_arrive_expect_tx(bar, 2 * p.group * p.tile_tokens * 128);
+                    for (int c = 0; c < 2; ++c) {
+                        tma_load_4d(smem_base + (2 * i + c) * CHUNK, &p.q, bar, c * 64, kv_head * p.group, (tile0 + i) * p.tile_tokens, entry);
+                    }
+                };
+                bool alive = true;
+                int chunk = 0;
+                auto acquire = [&](uint32_t& bar, uint64_t* counter) -> uint32_t {
+                    const int slot = chunk % RING;
+                    const int use = chunk / RING;
+                    if (use > 0 && !mbar_wait(smem_u32(&bars->ring_empty[slot]), (use - 1) & 1, abort_flag, &cross_forward_status)) {
+                        alive = false;
+                        return 0;
+                    }
+                    bar = smem_u32(counter != nullptr ? counter : &bars->ring_full[slot]);
+                    mbar_arrive_expect_tx(bar, CHUNK);
+                    ++chunk;
+                    return ring_smem + slot * CHUNK;
+                };
+                load_q(0);
+#pragma unroll 1
+                for (int j = 0; j < tile_count && alive; ++j) {
+                    const bool tail = tail_keys < TILE && j + 1 == tile_count;
+#pragma unroll 1
+                    for (int c = 0; c < 2 && alive; ++c) {
+                        uint32_t bar;
+                        const uint32_t dst = acquire(bar, nullptr);
+                        if (dst != 0) {
+                            tma_load_3d(dst, &p.k, bar, kv_head * HEAD + c * 64, j * TILE, entry);
+                        }
+                    }
+                    if (j == 0 && second) {
+                        load_q(1);
+                    }
+#pragma unroll 1
+                    for (int half = 0; half < 2 && alive; ++half) {
+                        uint32_t bar;
+                        const uint32_t dst = acquire(bar, tail ? &bars->tail_full[half] : nullptr);
+                        if (dst != 0) {
+                            tma_load_3d(dst, &p.v, bar, kv_head * HEAD, j * TILE + half * 64, entry);
+                            tma_load_3d(dst + CHUNK / 2, &p.v, bar, kv_head * HEAD + 64, j * TILE + half * 64, entry);
+                        }
+                    }
+                }
+            }
+        } else if (tile_count > 0) {
+            // ---- MMA: the whole warp runs the loop, the elected lane executes the instructions ----
+            const uint32_t leader = elect_one();
+            constexpr uint32_t IDESC_QK = make_idesc_bf16(TILE, TILE, false, false);
+            constexpr uint32_t IDESC_PV = make_idesc_bf16(TILE, HEAD, false, true);
+            const int tiles = second ? 2 : 1;
+            bool alive = true;
+            auto wait_chunk = [&](int chunk) -> uint32_t {
+                const int slot = chunk % RING;
+                if (!__all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->ring_full[slot]), (chunk / RING) & 1, abort_flag, &cross_forward_status))) {
+                    alive = false;
+                }
+                return ring_smem + slot * CHUNK;
+            };
+            auto issue_qk = [&](int i, int j) {
+                const uint32_t d = tmem_base + i * TILE;
+                for (int c = 0; c < 2; ++c) {
+                    const uint32_t k_chunk = wait_chunk(j * PER_TILE + c);
+                    if (!alive) {
+                        return;
+                    }
+                    tc_fence_after_sync();
+                    const uint32_t q_chunk = smem_base + (2 * i + c) * CHUNK;
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        mma_ss_elect(d, make_kmajor_desc(q_chunk + k * 32), make_kmajor_desc(k_chunk + k * 32), IDESC_QK, (c | k) != 0 ? 1U : 0U, leader);
+                    }
+                }
+                mma_commit_elect(smem_u32(&bars->s_full[i]), leader);
+                if (i + 1 == tiles) {
+                    for (int c = 0; c < 2; ++c) {
+                        mma_commit_elect(smem_u32(&bars->ring_empty[(j * PER_TILE + c) % RING]), leader);
+                    }
+                }
+            };
+            auto issue_pv = [&](int i, int j) {
+                const uint32_t d = tmem_base + 2 * TILE + i * HEAD;
+                const uint32_t p_tmem = tmem_base + i * TILE;
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t v_chunk = wait_chunk(j * PER_TILE + 2 + half);
+                    if (alive) {
+                        alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(half == 0 ? &bars->p_half[i] : &bars->p_full[i]), j & 1, abort_flag, &cross_forward_status));
+                    }
+                    if (!alive) {
+                        return;
+                    }
+                    tc_fence_after_sync();
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        mma_ts_elect(d, p_tmem + half * 32 + k * 8, make_smem_desc(v_chunk + k * 2048, CHUNK / 2, 1024), IDESC_PV,
+                                     (j | half | k) != 0 ? 1U : 0U, leader);
+                    }
+                }
+                if (i + 1 == tiles) {
+                    for (int half = 0; half < 2; ++half) {
+                        mma_commit_elect(smem_u32(&bars->ring_empty[(j * PER_TILE + 2 + half) % RING]), leader);
+                    }
+                }
+            };
+            for (int i = 0; i < tiles && alive; ++i) {
+                alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->q_full[i]), 0, abort_flag, &cross_forward_status));
+                if (alive) {
+                    issue_qk(i, 0);
+                }
+            }
+            for (int j = 0; j < tile_count && alive; ++j) {
+                for (int i = 0; i < tiles && alive; ++i) {
+                    issue_pv(i, j);
+                    if (!alive) {
+                        break;
+                    }
+                    if (j + 1 < tile_count) {
+                        issue_qk(i, j + 1);
+                    } else {
+                        mma_commit_elect(smem_u32(&bars->s_full[i]), leader);       // O_i is final
+                    }
+                }
+            }
+        }
+    } else {
+        // ---- softmax and output: a thread to a row ----
+        reg_alloc<REG_HI>();
+        const int i = warp / 4;
+        const int r = threadIdx.x % TILE;
+        const uint32_t lane_base = static_cast<uint32_t>((warp % 4) * 32) << 16;
+        const uint32_t s_tmem = tmem_base + lane_base + i * TILE;
+        const uint32_t o_tmem = tmem_base + lane_base + 2 * TILE + i * HEAD;
+        const int token = (tile0 + i) * p.tile_tokens + r / p.group;
+        const bool valid = r < p.tile_tokens * p.group && token < p.tokens;
+        const int count = i == 0 || second ? tile_count : 0;
+        float* lse = p.lse + (static_cast<size_t>(entry) * p.heads + kv_head * p.group + r % p.group) * p.tokens + token;
+        float m_ref = 0.0F;
+        float l_sum = 0.0F;
+        bool alive = true;
+
+        for (int j = 0; j < count; ++j) {
+            alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->s_full[i]), j & 1, abort_flag, &cross_forward_status));
+            if (!alive) {
+                break;
+            }
+            tc_fence_after_sync();
+            uint32_t sb[TILE];
+#pragma unroll
+            for (int c = 0; c < TILE / 32; ++c) {
+                tmem_ld_x32(s_tmem + c * 32, sb + c * 32);
+            }
+            tmem_wait_ld();
+            if (j == count - 1) {
+                const int left = length - j * TILE;
+#pragma unroll
+                for (int n = 0; n < TILE; ++n) {
+                    sb[n] = n < left ? sb[n] : 0xff800000U;
+                }
+            }
+            float mx0 = __uint_as_float(sb[0]), mx1 = __uint_as_float(sb[1]), mx2 = __uint_as_float(sb[2]), mx3 = __uint_as_float(sb[3]);
+#pragma unroll
+            for (int n = 4; n + 7 < TILE; n += 8) {
+                mx0 = max3(mx0, __uint_as_float(sb[n]), __uint_as_float(sb[n + 1]));
+                mx1 = max3(mx1, __uint_as_float(sb[n + 2]), __uint_as_float(sb[n + 3]));
+                mx2 = max3(mx2, __uint_as_float(sb[n + 4]), __uint_as_float(sb[n + 5]));
+                mx3 = max3(mx3, __uint_as_float(sb[n + 6]), __uint_as_float(sb[n + 7]));
+            }
+            mx0 = max3(mx0, __uint_as_float(sb[TILE - 4]), __uint_as_float(sb[TILE - 3]));
+            mx1 = max3(mx1, __uint_as_float(sb[TILE - 2]), __uint_as_float(sb[TILE - 1]));
+            const float tile_max = fmaxf(fmaxf(mx0, mx1), fmaxf(mx2, mx3));
+            if (j == 0) {
+                m_ref = tile_max;
+            } else {
+                const bool grow = (tile_max - m_ref) * p.scale_log2 > RESCALE_THRESHOLD;
+                if (__any_sync(0xffffffffU, grow)) {
+                    float alpha = 1.0F;
+                    if (grow) {
+                        alpha = exp2_approx((m_ref - tile_max) * p.scale_log2);
+                        m_ref = tile_max;
+                        l_sum *= alpha;
+                    }
+                    // S_i(j) complete implies P_i(j-1) V complete: O_i is quiescent here
+#pragma unroll
+                    for (int c = 0; c < HEAD / 32; ++c) {
+                        uint32_t o[32];
+                        tmem_ld_x32(o_tmem + c * 32, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int e = 0; e < 32; ++e) {
+                            o[e] = __float_as_uint(__uint_as_float(o[e]) * alpha);
+                        }
+                        tmem_st_x32(o_tmem + c * 32, o);
+                    }
+                }
+            }
+            const float bias = -m_ref * p.scale_log2;
+            float2 sums = make_float2(0.0F, 0.0F);
+            const float2 scale2 = make_float2(p.scale_log2, p.scale_log2);
+            const float2 bias2 = make_float2(bias, bias);
+#pragma unroll
+            for (int c = 0; c < TILE / 32; ++c) {
+                uint32_t packed[16];
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const float2 x = fma2(make_float2(__uint_as_float(sb[c * 32 + 2 * e]), __uint_as_float(sb[c * 32 + 2 * e + 1])), scale2, bias2);
+                    const float2 pr = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                    sums = add2(sums, pr);
+                    packed[e] = pack_bf16x2(pr.x, pr.y);
+                }
+                tmem_st_x16(s_tmem + c * 16, packed);
+                if (c == 1) {
+                    tmem_wait_st();
+                    tc_fence_before_sync();
+                    mbar_arrive(smem_u32(&bars->p_half[i]));
+                }
+            }
+            l_sum += sums.x + sums.y;
+            tmem_wait_st();
+            tc_fence_before_sync();
+            mbar_arrive(smem_u32(&bars->p_full[i]));
+        }
+        const bool active = i == 0 || second;
+        if (alive && count > 0) {
+            alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->s_full[i]), count & 1, abort_flag, &cross_forward_status));
+        }
+        if (alive && active) {
+            // rows of 64 columns into the tile's Q chunks (idle by now), from where a TMA store takes them
+            tc_fence_after_sync();
+            const float inverse = count > 0 ? 1.0F / l_sum : 0.0F;
+#pragma unroll
+            for (int c = 0; c < HEAD / 32; ++c) {
+                uint32_t o[32];
+                if (count > 0) {
+                    tmem_ld_x32(o_tmem + c * 32, o);
+                    tmem_wait_ld();
+                } else {
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        o[e] = 0;
+                    }
+                }
+                uint8_t* row = smem + (2 * i + c / 2) * CHUNK + r * 128;
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    uint4 vec;
+                    vec.x = pack_bf16x2(__uint_as_float(o[8 * u]) * inverse, __uint_as_float(o[8 * u + 1]) * inverse);
+                    vec.y = pack_bf16x2(__uint_as_float(o[8 * u + 2]) * inverse, __uint_as_float(o[8 * u + 3]) * inverse);
+                    vec.z = pack_bf16x2(__uint_as_float(o[8 * u + 4]) * inverse, __uint_as_float(o[8 * u + 5]) * inverse);
+                    vec.w = pack_bf16x2(__uint_as_float(o[8 * u + 6]) * inverse, __uint_as_float(o[8 * u + 7]) * inverse);
+                    *reinterpret_cast<uint4*>(row + ((((c % 2) * 4 + u) ^ (r & 7)) * 16)) = vec;
+                }
+            }
+            if (valid) {
+                *lse = count > 0 ? m_ref * p.scale + logf(l_sum) : -INFINITY;
+            }
+            fence_proxy_async_smem();
+            mbar_arrive(smem_u32(&bars->staged[i]));
+            if (r == 0 && mbar_wait(smem_u32(&bars->staged[i]), 0, abort_flag, &cross_forward_status)) {
+                for (int c = 0; c < 2; ++c) {
+                    tma_store_4d(&p.out, smem_base + (2 * i + c) * CHUNK, c * 64, kv_head * p.group, (tile0 + i) * p.tile_tokens, entry);
+                }
+                tma_store_commit();
+                tma_store_wait_read();
+            }
+        }
+    }
+
+    // ---- teardown: every path reaches this point ----
+    __syncwarp();
+    tc_fence_before_sync();
+    __syncthreads();
+    if (*abort_flag != 0) {
+        for (int k = 0; k < 64; ++k) {
+            __nanosleep(1000);
+        }
+    }
+    if (warp == MMA_WARP) {
+        tc_fence_after_sync();
+        tmem_dealloc(tmem_base, TMEM_COLUMNS);
+    }
+}
+
+void configure() {
+    static bool done[16] = {};
+    int device = 0;
+    CUDA_CHECK(cudaGetDevice(&device));
+    if (device < 16 && done[device]) {
+        return;
+    }
+    CUDA_CHECK(cudaFuncSetAttribute(cross_forward_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+    if (device < 16) {
+        done[device] = true;
+    }
+}
+
+// Rows to a key head up to which flash_decode.cu's kernels take the call.
+constexpr long long FEW_ROWS = 32;
+
+}  // namespace
+
+namespace internal {
+
+void check_flash_cross_shape(int batch_size, int query_length, int key_length, int query_heads, int key_value_heads, int head_size, float scale) {
+    if (head_size != HEAD) {
+        throw std::invalid_argument("flash cross attention requires head_size 128");
+    }
+    if (batch_size <= 0 || query_length <= 0 || key_length <= 0) {
+        throw std::invalid_argument("flash cross attention requires positive batch and lengths");
+    }
+    if (query_heads <= 0 || key_value_heads <= 0 || query_heads % key_value_heads != 0) {
+        throw std::invalid_argument("flash cross attention requires query_heads to be divisible by key_value_heads");
+    }
+    if (query_heads / key_value_heads > 64) {
+        throw std::invalid_argument("flash cross attention takes at most 64 query heads to a key head");
+    }
+    if (!(scale > 0.0F)) {
+        throw std::invalid_argument("flash cross attention requires a positive softmax scale");
+    }
+    if (static_cast<long long>(batch_size) * query_length > 0x7fffffffLL || static_cast<long long>(batch_size) * key_length > 0x7fffffffLL ||
+        query_length > (1 << 30) || key_length > (1 << 30) || static_cast<long long>(query_length) * query_heads > 0x7fffffffLL ||
+        query_heads > 65535 || batch_size > 65535) {
+        throw std::invalid_argument("flash cross attention shape exceeds the supported index range");
+    }
+}
+
+int cross_forward_device_status(bool reset) {
+    int status = 0;
+    CUDA_CHECK(cudaDeviceSynchronize());
+    CUDA_CHECK(cudaMemcpyFromSymbol(&status, cross_forward_status, sizeof(int)));
+    if (reset && status != 0) {
+        const int zero = 0;
+        CUDA_CHECK(cudaMemcpyToSymbol(cross_forward_status, &zero, sizeof(int)));
+    }
+    return status;
+}
+
+}  // namespace internal
+
+std::size_t flash_cross_forward_workspace_bytes(int batch_size, int query_length, int key_length, int query_heads, int key_value_heads) {
+    if (batch_size <= 0 || query_length <= 0 || key_length <= 0 || query_heads <= 0 || key_value_heads <= 0) {
+        return 0;
+    }
+    const long long rows = static_cast<long long>(query_length) * (query_heads / key_value_heads);
+    return rows <= FEW_ROWS ? internal::few_rows_workspace_bytes(rows) : 0;
+}
+
+void flash_cross_forward_cuda(__nv_bfloat16* output, float* logsumexp, const __nv_bfloat16* query, const __nv_bfloat16* key,
+                              const __nv_bfloat16* value, const int* key_lengths, void* workspace, std::size_t workspace_bytes, int batch_size,
+                              int query_length, int key_length, int query_heads, int key_value_heads, int head_size, float scale,
+                              cudaStream_t stream) {
+    internal::check_flash_cross_shape(batch_size, query_length, key_length, query_heads, key_value_heads, head_size, scale);
+    internal::check_flash_pointers({output, query, key, value}, {logsumexp});
+    if (key_lengths != nullptr) {
+        internal::check_flash_pointers({}, {key_lengths});
+    }
+    const std::size_t needed = flash_cross_forward_workspace_bytes(batch_size, query_length, key_length, query_heads, key_value_heads);
+    if (needed > 0) {
+        internal::check_flash_pointers({workspace}, {});
+        if (workspace_bytes < needed) {
+            throw std::invalid_argument("flash cross attention workspace is too small");
+        }
+    }
+    const int group = query_heads / key_value_heads;
+    if (static_cast<long long>(query_length) * group <= FEW_ROWS) {
+        internal::launch_few_rows_cross(output, logsumexp, query, key, value, key_lengths, workspace, batch_size, query_length, key_length, query_heads,
+                                        key_value_heads, scale, stream);
+        return;
+    }
+    CrossForwardParams p{};
+    p.tile_tokens = TILE / group;
+    p.q = make_bf16_group_rows_map(query, batch_size, query_length, query_heads, group, p.tile_tokens);
+    p.out = make_bf16_group_rows_map(output, batch_size, query_length, query_heads, group, p.tile_tokens);
+    p.k = make_bf16_batched_tile_map(key, batch_size, key_length, static_cast<std::uint64_t>(key_value_heads) * HEAD, TILE);
+    p.v = make_bf16_batched_tile_map(value, batch_size, key_length, static_cast<std::uint64_t>(key_value_heads) * HEAD, 64);
+    p.lse = logsumexp;
+    p.lengths = key_lengths;
+    p.tokens = query_length;
+    p.keys = key_length;
+    p.heads = query_heads;
+    p.group = group;
+    p.scale = scale;
+    p.scale_log2 = scale * LOG2E;
+    configure();
+    const int row_tiles = (query_length + p.tile_tokens - 1) / p.tile_tokens;
+    launch_chained(cross_forward_kernel, dim3((row_tiles + 1) / 2, key_value_heads, batch_size), dim3(THREADS), SMEM_BYTES, stream, p);
+}
+
+}  // namespace dscuda

@@ -195,6 +195,14 @@ __device__ __forceinline__ void tma_load_3d(uint32_t smem_dst, const void* tenso
         : "memory");
 }
 
+// 4-D form.
+__device__ __forceinline__ void tma_load_4d(uint32_t smem_dst, const void* tensor_map, uint32_t bar, int x, int y, int z, int w) {
+    asm volatile(
+        "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+        ::"r"(smem_dst), "l"(tensor_map), "r"(bar), "r"(x), "r"(y), "r"(z), "r"(w)
+        : "memory");
+}
+
 // The same for a CTA pair (cta_group::2): lands in this CTA's shared memory and signals the barrier at `cluster_bar`, which
 // may be the other CTA's (map_to_cta).
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t smem_dst, const void* tensor_map, uint32_t cluster_bar, int x, int y) {

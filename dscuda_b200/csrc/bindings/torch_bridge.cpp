@@ -9,6 +9,7 @@
 #include "dscuda_c_api.h"
 
 #include <ATen/Functions.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -17,9 +18,11 @@
 
 #include <Python.h>
 
+#include <algorithm>
 #include <optional>
 #include <stdexcept>
 #include <string>
+#include <vector>
 
 namespace {
 
@@ -548,13 +551,343 @@ DSCUDA_FUNCTION(flash_forward) {
     });
 }
 
+// ---- grouped-query operators around flash_forward (dscuda_b200/flash.py) ----------------------
+// Inputs of these calls are checked for device, type and shape as well; work goes to the inputs' device and its current stream.
+void expect_input(const Tensor& t, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes, const char* what) {
+    if (t.device() != like.device()) {
+        fail(PyExc_ValueError, std::string(what) + " is on another device than the other inputs");
+    }
+    if (t.scalar_type() != type) {
+        fail(PyExc_ValueError, std::string(what) + " has the wrong dtype");
+    }
+    if (t.sizes() != sizes) {
+        std::string wanted;
+        for (const int64_t size : sizes) {
+            wanted += (wanted.empty() ? "" : ", ") + std::to_string(size);
+        }
+        fail(PyExc_ValueError, std::string(what) + " has another shape than [" + wanted + "]");
+    }
+}
+
+// A CUDA tensor [..., heads, width] in bf16 whose heads are contiguous and whose rows lie `stride` elements apart (a part of a fused
+// projection); null for None.
+struct Rows {
+    const Tensor* tensor = nullptr;
+    long long stride = 0;
+};
+
+Rows strided_rows(PyObject* object, const char* what) {
+    if (!THPVariable_Check(object)) {
+        fail(PyExc_TypeError, std::string("expected a torch tensor, got ") + Py_TYPE(object)->tp_name);
+    }
+    const Tensor& t = THPVariable_Unpack(object);
+    if (!t.is_cuda()) {
+        fail(PyExc_RuntimeError, "dscuda_b200 runs on CUDA tensors only; there is no CPU path");
+    }
+    if (t.scalar_type() != at::kBFloat16) {
+        fail(PyExc_ValueError, std::string(what) + " has the wrong dtype");
+    }
+    if (t.dim() < 3 || t.numel() == 0) {
+        fail(PyExc_ValueError, std::string(what) + " is a tensor [..., heads, width] that is not empty");
+    }
+    const int64_t dims = t.dim(), heads = t.size(-2), width = t.size(-1);
+    if ((width > 1 && t.stride(-1) != 1) || (heads > 1 && t.stride(-2) != width)) {
+        fail(PyExc_ValueError, std::string(what) + ": the heads of a token must be contiguous");
+    }
+    Rows rows{&t, heads * width};
+    int64_t expected = -1;              // stride that the next dimension outwards must have
+    for (int64_t d = dims - 3; d >= 0; --d) {
+        if (t.size(d) == 1) {
+            continue;
+        }
+        if (expected < 0) {
+            rows.stride = t.stride(d);
+        } else if (t.stride(d) != expected) {
+            fail(PyExc_ValueError, std::string(what) + ": tokens must lie the same distance apart");
+        }
+        expected = t.stride(d) * t.size(d);
+    }
+    return rows;
+}
+
+struct OnDevice {
+    c10::cuda::CUDAGuard guard;
+    void* stream;
+    explicit OnDevice(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
+};
+
+bool truth(PyObject* object) {
+    const int value = PyObject_IsTrue(object);
+    if (value < 0) {
+        throw python_error();
+    }
+    return value != 0;
+}
+
+// query, key, positions, sections, theta, restart, inverse, query_out, key_out -> query_out, key_out
+DSCUDA_FUNCTION(flash_rope) {
+    return guarded([&] {
+        expect_arguments(count, 9);
+        Rows in[2], out[2];
+        const char* names[2] = {"the query", "the key"};
+        for (int i = 0; i < 2; ++i) {
+            if (args[i] != Py_None) {
+                in[i] = strided_rows(args[i], names[i]);
+            }
+        }
+        const Tensor* anchor = in[0].tensor != nullptr ? in[0].tensor : in[1].tensor;
+        if (anchor == nullptr) {
+            fail(PyExc_ValueError, "nothing to rotate");
+        }
+        const long long rows = anchor->numel() / (anchor->size(-2) * anchor->size(-1));
+        const int width = extent(*anchor, -1);
+        if (in[0].tensor != nullptr && in[1].tensor != nullptr) {
+            const Tensor& key = *in[1].tensor;
+            if (key.device() != anchor->device()) {
+                fail(PyExc_ValueError, "the key is on another device than the other inputs");
+            }
+            if (key.dim() != anchor->dim() || key.size(-1) != width || key.sizes().slice(0, key.dim() - 2) != anchor->sizes().slice(0, key.dim() - 2)) {
+                fail(PyExc_ValueError, "query and key have different tokens or widths");
+            }
+        }
+        const THPObjectPtr items(PySequence_Fast(args[3], "sections is a sequence of numbers"));
+        if (!items) {
+            throw python_error();
+        }
+        std::vector<int> sections;
+        for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(items.get()); ++i) {
+            sections.push_back(static_cast<int>(integer(PySequence_Fast_GET_ITEM(items.get(), i))));
+        }
+        const Tensor& positions = tensor(args[2]);
+        if (positions.device() != anchor->device() || positions.scalar_type() != at::kInt) {
+            fail(PyExc_ValueError, "positions is an int32 tensor on the device of the other inputs");
+        }
+        if (positions.dim() < 1 || positions.size(0) != static_cast<int64_t>(sections.size()) || positions.numel() != rows * static_cast<int64_t>(sections.size())) {
+            fail(PyExc_ValueError, "positions holds one row for each section, with one number for each token");
+        }
+        const float theta = number(args[4]);
+        const bool restart = truth(args[5]), inverse = truth(args[6]);
+        Tensor made[2];
+        for (int i = 0; i < 2; ++i) {
+            if (in[i].tensor == nullptr) {
+                if (args[7 + i] != Py_None) {
+                    fail(PyExc_ValueError, std::string(names[i]) + " is missing, but its output is given");
+                }
+                continue;
+            }
+            if (args[7 + i] != Py_None) {
+                out[i] = strided_rows(args[7 + i], "an output");
+                expect_input(*out[i].tensor, *anchor, at::kBFloat16, in[i].tensor->sizes(), "an output");
+            } else {
+                made[i] = new_tensor(in[i].tensor->sizes(), *anchor, at::kBFloat16);
+                out[i] = {&made[i], made[i].size(-2) * made[i].size(-1)};
+            }
+        }
+        const int heads[2] = {in[0].tensor != nullptr ? extent(*in[0].tensor, -2) : 0, in[1].tensor != nullptr ? extent(*in[1].tensor, -2) : 0};
+        const OnDevice on(*anchor);
+        checked(dscuda_flash_last_error, [&] {
+            return dscuda_flash_rope(pointer(out[0].tensor), pointer(out[1].tensor), pointer(in[0].tensor), pointer(in[1].tensor), int_pointer(&positions), rows,
+                                     heads[0], heads[1], width, out[0].stride, out[1].stride, in[0].stride, in[1].stride, static_cast<int>(sections.size()),
+                                     sections.data(), restart, inverse, theta, on.stream);
+        });
+        PyObject* result = PyTuple_New(2);
+        if (result == nullptr) {
+            throw python_error();
+        }
+        for (int i = 0; i < 2; ++i) {
+            PyObject* item = made[i].defined() ? wrap(made[i]) : args[7 + i];
+            if (!made[i].defined()) {
+                Py_INCREF(item);
+            }
+            PyTuple_SET_ITEM(result, i, item);
+        }
+        return result;
+    });
+}
+
+// The four tensors of an 8-bit cache.
+struct FlashCache {
+    const Tensor &keys, &values, &key_scale, &value_scale;
+    int blocks, heads, page, width, type;
+};
+
+FlashCache flash_cache(PyObject* const* args) {
+    const Tensor &keys = tensor(args[0], 4), &values = tensor(args[1]), &key_scale = tensor(args[2]), &value_scale = tensor(args[3]);
+    const bool int8 = keys.scalar_type() == at::kChar;
+    if (!int8 && keys.scalar_type() != at::kFloat8_e4m3fn) {
+        fail(PyExc_ValueError, "the cache holds int8 or float8_e4m3fn codes [blocks, heads, page, 128]");
+    }
+    expect_input(values, keys, keys.scalar_type(), keys.sizes(), "the value cache");
+    expect_input(key_scale, keys, at::kFloat, {keys.size(0), keys.size(1)}, "the key scales");
+    expect_input(value_scale, keys, at::kFloat, {keys.size(0), keys.size(1)}, "the value scales");
+    return {keys, values, key_scale, value_scale, extent(keys, 0), extent(keys, 1), extent(keys, 2), extent(keys, 3), int8 ? 0 : 1};
+}
+
+// key_cache, value_cache, key_scale, value_scale, key, value, block_table, start_positions, token_counts
+DSCUDA_FUNCTION(flash_cache_append) {
+    return guarded([&] {
+        expect_arguments(count, 9);
+        const FlashCache cache = flash_cache(args);
+        const Rows key = strided_rows(args[4], "the key"), value = strided_rows(args[5], "the value");
+        if (key.tensor->dim() != 4) {
+            fail(PyExc_ValueError, "the key is a tensor [batch, tokens, heads, 128]");
+        }
+        const int64_t b = key.tensor->size(0), t = key.tensor->size(1);
+        expect_input(*key.tensor, cache.keys, at::kBFloat16, {b, t, cache.heads, cache.width}, "the key");
+        expect_input(*value.tensor, cache.keys, at::kBFloat16, {b, t, cache.heads, cache.width}, "the value");
+        const Tensor& table = tensor(args[6], 2);
+        expect_input(table, cache.keys, at::kInt, {b, table.size(1)}, "the block table");
+        const Tensor *starts = optional_tensor(args[7]), *counts = optional_tensor(args[8]);
+        if (starts != nullptr) {
+            expect_input(*starts, cache.keys, at::kInt, {b}, "start_positions");
+        }
+        if (counts != nullptr) {
+            expect_input(*counts, cache.keys, at::kInt, {b}, "token_counts");
+        }
+        const OnDevice on(cache.keys);
+        checked(dscuda_flash_last_error, [&] {
+            return dscuda_flash_cache_append(pointer(cache.keys), pointer(cache.values), static_cast<float*>(pointer(cache.key_scale)),
+                                             static_cast<float*>(pointer(cache.value_scale)), pointer(key.tensor), pointer(value.tensor), int_pointer(&table),
+                                             int_pointer(starts), int_pointer(counts), static_cast<int>(b), static_cast<int>(t), cache.heads, cache.width,
+                                             key.stride, value.stride, cache.page, extent(table, 1), cache.blocks, cache.type, on.stream);
+        });
+        Py_RETURN_NONE;
+    });
+}
+
+// query, key_cache, value_cache, key_scale, value_scale, block_table, cache_lengths, scale, workspace, output, lse -> output, lse
+DSCUDA_FUNCTION(flash_decode) {
+    return guarded([&] {
+        expect_arguments(count, 11);
+        const Tensor& query = tensor(args[0], 4);
+        const FlashCache cache = flash_cache(args + 1);
+        const int64_t b = query.size(0), t = query.size(1), hq = query.size(2);
+        expect_input(query, cache.keys, at::kBFloat16, {b, t, hq, cache.width}, "the query");
+        const Tensor &table = tensor(args[5], 2), &lengths = tensor(args[6]);
+        expect_input(table, query, at::kInt, {b, table.size(1)}, "the block table");
+        expect_input(lengths, query, at::kInt, {b}, "cache_lengths");
+        const float scale = number(args[7]);
+        const size_t bytes = dscuda_flash_decode_workspace_bytes(static_cast<int>(t), static_cast<int>(hq), cache.heads);
+        const Tensor* workspace_given = optional_workspace(args[8], query, bytes);
+        const Tensor *output_given = optional_output(args[9], query, at::kBFloat16, query.numel(), "the output"),
+                     *lse_given = optional_output(args[10], query, at::kFloat, b * hq * t, "the LSE");
+        Tensor workspace = workspace_given != nullptr ? *workspace_given : new_tensor({static_cast<int64_t>(bytes)}, query, at::kByte);
+        Tensor output = output_given != nullptr ? *output_given : new_like(query);
+        Tensor lse = lse_given != nullptr ? *lse_given : new_tensor({b, hq, t}, query, at::kFloat);
+        const OnDevice on(query);
+        checked(dscuda_flash_last_error, [&] {
+            return dscuda_flash_decode(pointer(output), static_cast<float*>(pointer(lse)), pointer(query), pointer(cache.keys), pointer(cache.values),
+                                       static_cast<const float*>(pointer(cache.key_scale)), static_cast<const float*>(pointer(cache.value_scale)),
+                                       int_pointer(&table), int_pointer(&lengths), pointer(workspace), workspace.nbytes(), static_cast<int>(b),
+                                       static_cast<int>(t), static_cast<int>(hq), cache.heads, cache.width, cache.page, extent(table, 1), cache.blocks,
+                                       cache.type, scale, on.stream);
+        });
+        return tuple(output, lse);
+    });
+}
+
+struct CrossShape {
+    int batch, queries, keys, heads, kv_heads, width;
+    const Tensor* lengths;
+};
+
+CrossShape cross_shape(const Tensor& query, const Tensor& key, const Tensor& value, PyObject* lengths) {
+    expect_input(query, query, at::kBFloat16, query.sizes(), "the query");
+    expect_input(key, query, at::kBFloat16, {query.size(0), key.size(1), key.size(2), query.size(3)}, "the key");
+    expect_input(value, query, at::kBFloat16, key.sizes(), "the value");
+    const Tensor* given = optional_tensor(lengths);
+    if (given != nullptr) {
+        expect_input(*given, query, at::kInt, {query.size(0)}, "key_lengths");
+    }
+    return {extent(query, 0), extent(query, 1), extent(key, 1), extent(query, 2), extent(key, 2), extent(query, 3), given};
+}
+
+// query, key, value, scale, key_lengths, workspace, output, lse -> output, lse
+DSCUDA_FUNCTION(flash_cross_forward) {
+    return guarded([&] {
+        expect_arguments(count, 8);
+        const Tensor &query = tensor(args[0], 4), &key = tensor(args[1], 4), &value = tensor(args[2], 4);
+        const float scale = number(args[3]);
+        const CrossShape n = cross_shape(query, key, value, args[4]);
+        const size_t bytes = dscuda_flash_cross_forward_workspace_bytes(n.batch, n.queries, n.keys, n.heads, n.kv_heads);
+        const Tensor* workspace_given = optional_workspace(args[5], query, bytes);
+        const Tensor *output_given = optional_output(args[6], query, at::kBFloat16, query.numel(), "the output"),
+                     *lse_given = optional_output(args[7], query, at::kFloat, query.numel() / std::max(1, n.width), "the LSE");
+        Tensor workspace;
+        if (workspace_given != nullptr) {
+            workspace = *workspace_given;
+        } else if (bytes > 0) {
+            workspace = new_tensor({static_cast<int64_t>(bytes)}, query, at::kByte);
+        }
+        Tensor output = output_given != nullptr ? *output_given : new_like(query);
+        Tensor lse = lse_given != nullptr ? *lse_given : new_tensor({n.batch, n.heads, n.queries}, query, at::kFloat);
+        const OnDevice on(query);
+        checked(dscuda_flash_last_error, [&] {
+            return dscuda_flash_cross_forward(pointer(output), static_cast<float*>(pointer(lse)), pointer(query), pointer(key), pointer(value),
+                                              int_pointer(n.lengths), workspace.defined() ? pointer(workspace) : nullptr,
+                                              workspace.defined() ? workspace.nbytes() : 0, n.batch, n.queries, n.keys, n.heads, n.kv_heads, n.width, scale,
+                                              on.stream);
+        });
+        return tuple(output, lse);
+    });
+}
+
+// dout, output, lse, query, key, value, scale, key_lengths, workspace, grads -> dquery, dkey, dvalue
+DSCUDA_FUNCTION(flash_cross_backward) {
+    return guarded([&] {
+        expect_arguments(count, 10);
+        const Tensor &dout = tensor(args[0], 4), &output = tensor(args[1]), &lse = tensor(args[2]), &query = tensor(args[3], 4), &key = tensor(args[4], 4),
+                     &value = tensor(args[5], 4);
+        const float scale = number(args[6]);
+        const CrossShape n = cross_shape(query, key, value, args[7]);
+        expect_input(dout, query, at::kBFloat16, query.sizes(), "dout");
+        expect_input(output, query, at::kBFloat16, query.sizes(), "the output");
+        expect_input(lse, query, at::kFloat, {n.batch, n.heads, n.queries}, "the LSE");
+        const size_t bytes = dscuda_flash_cross_backward_workspace_bytes(n.batch, n.queries, n.keys, n.heads, n.kv_heads);
+        const Tensor* workspace_given = optional_workspace(args[8], query, bytes);
+        Tensor grads[3];
+        if (args[9] == Py_None) {
+            grads[0] = new_like(query);
+            grads[1] = new_like(key);
+            grads[2] = new_like(value);
+        } else {
+            const THPObjectPtr items(PySequence_Fast(args[9], "grads is a sequence of three tensors"));
+            if (!items) {
+                throw python_error();
+            }
+            if (PySequence_Fast_GET_SIZE(items.get()) != 3) {
+                fail(PyExc_ValueError, "grads is a sequence of three tensors");
+            }
+            const Tensor* like[3] = {&query, &key, &value};
+            const char* names[3] = {"dquery", "dkey", "dvalue"};
+            for (int i = 0; i < 3; ++i) {
+                const Tensor* grad = optional_output(PySequence_Fast_GET_ITEM(items.get(), i), query, at::kBFloat16, like[i]->numel(), names[i]);
+                if (grad == nullptr) {
+                    fail(PyExc_TypeError, "grads is a sequence of three tensors");
+                }
+                grads[i] = *grad;
+            }
+        }
+        Tensor workspace = workspace_given != nullptr ? *workspace_given : new_tensor({static_cast<int64_t>(bytes)}, query, at::kByte);
+        const OnDevice on(query);
+        checked(dscuda_flash_last_error, [&] {
+            return dscuda_flash_cross_backward(pointer(grads[0]), pointer(grads[1]), pointer(grads[2]), pointer(dout), pointer(output),
+                                               static_cast<const float*>(pointer(lse)), pointer(query), pointer(key), pointer(value), int_pointer(n.lengths),
+                                               pointer(workspace), workspace.nbytes(), n.batch, n.queries, n.keys, n.heads, n.kv_heads, n.width, scale,
+                                               on.stream);
+        });
+        return tuple(grads[0], grads[1], grads[2]);
+    });
+}
+
 #define DSCUDA_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 
 PyMethodDef methods[] = {
     DSCUDA_METHOD(mla_forward),      DSCUDA_METHOD(mla_backward),     DSCUDA_METHOD(mla_decode),           DSCUDA_METHOD(cache_append),
     DSCUDA_METHOD(cache_append_fp8), DSCUDA_METHOD(rope_apply),       DSCUDA_METHOD(cache_dequantize_fp8), DSCUDA_METHOD(up_project),
     DSCUDA_METHOD(absorb_query),     DSCUDA_METHOD(unabsorb_output),  DSCUDA_METHOD(prefill_forward),      DSCUDA_METHOD(prefill_backward),
-    DSCUDA_METHOD(flash_forward),    {nullptr, nullptr, 0, nullptr},
+    DSCUDA_METHOD(flash_forward),    DSCUDA_METHOD(flash_rope),       DSCUDA_METHOD(flash_cache_append),   DSCUDA_METHOD(flash_decode),
+    DSCUDA_METHOD(flash_cross_forward), DSCUDA_METHOD(flash_cross_backward), {nullptr, nullptr, 0, nullptr},
 };
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_dscuda_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

@@ -75,6 +75,28 @@ CUtensorMap make_bf16_batched_tile_map(const void* base, std::uint64_t batch, st
     return map;
 }
 
+CUtensorMap make_bf16_group_rows_map(const void* base, std::uint64_t batch, std::uint64_t tokens, std::uint64_t heads, std::uint32_t group,
+                                     std::uint32_t box_tokens) {
+    if ((reinterpret_cast<std::uintptr_t>(base) & 15U) != 0) {
+        throw std::invalid_argument("tensor base must be 16-byte aligned");
+    }
+    if (batch == 0 || tokens == 0 || heads == 0 || group == 0 || group > 256 || box_tokens == 0 || box_tokens > 256) {
+        throw std::invalid_argument("empty tensor or bad box");
+    }
+    CUtensorMap map;
+    const cuuint64_t dims[4] = {128, heads, tokens, batch};
+    const cuuint64_t strides[3] = {256, heads * 256, tokens * heads * 256};
+    const cuuint32_t box[4] = {64, group, box_tokens, 1};
+    const cuuint32_t element_strides[4] = {1, 1, 1, 1};
+    const CUresult result = encode_entry_point()(&map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4, const_cast<void*>(base), dims, strides, box, element_strides,
+                                                 CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                                                 CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (result != CUDA_SUCCESS) {
+        throw std::runtime_error("cuTensorMapEncodeTiled (group rows) failed with code " + std::to_string(static_cast<int>(result)));
+    }
+    return map;
+}
+
 CUtensorMap make_bf16_chunked_map(const void* base, std::uint64_t rows, std::uint32_t chunks, std::uint64_t row_stride_elements,
                                   std::uint32_t box_rows, std::uint32_t box_chunks) {
     if ((reinterpret_cast<std::uintptr_t>(base) & 15U) != 0 || (row_stride_elements * 2) % 16 != 0) {

@@ -20,6 +20,12 @@ CUtensorMap make_bf16_tile_map(const void* base, std::uint64_t rows, std::uint64
 // Rows past the entry's last one read as zero, not as the next entry's.
 CUtensorMap make_bf16_batched_tile_map(const void* base, std::uint64_t batch, std::uint64_t rows, std::uint64_t cols, std::uint32_t box_rows);
 
+// Heads of width 128, [batch][tokens][heads][128] contiguous, as the rows of groups: box {64, group, box_tokens, 1} at
+// {column, first head of the group, token, entry} is group * box_tokens rows of shared memory, row = token * group + head.  Tokens past the
+// entry's last one read as zero; stored rows of such tokens are clipped.
+CUtensorMap make_bf16_group_rows_map(const void* base, std::uint64_t batch, std::uint64_t tokens, std::uint64_t heads, std::uint32_t group,
+                                     std::uint32_t box_tokens);
+
 // The same rows seen as [chunk][row][64 elements]: `chunks` consecutive 64-column chunks of a row are
 // 128 bytes apart, rows `row_stride_elements` apart.  One load of a box {64, box_rows, box_chunks} at
 // coordinates {0, row, chunk} lands in shared memory chunk after chunk, each a [box_rows x 128 byte]

@@ -17,7 +17,7 @@ import re
 import sys
 
 ROOT = pathlib.Path(__file__).resolve().parents[1]
-P, I, F = ctypes.c_void_p, ctypes.c_int, ctypes.c_float
+P, I, F, L, Z = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong, ctypes.c_size_t
 
 # name -> (argument types, result type); the order is the C declaration order.
 MLA_SYMBOLS = {
@@ -47,6 +47,14 @@ MLA_SYMBOLS = {
 FLASH_SYMBOLS = {
     "dscuda_flash_last_error": ([], ctypes.c_char_p),
     "dscuda_flash_forward": ([P] * 5 + [I] * 5 + [F, P], I),
+    "dscuda_flash_rope": ([P] * 5 + [L] + [I] * 3 + [L] * 4 + [I, P, I, I, F, P], I),
+    "dscuda_flash_cache_append": ([P] * 9 + [I] * 4 + [L] * 2 + [I] * 4 + [P], I),
+    "dscuda_flash_decode_workspace_bytes": ([I] * 3, Z),
+    "dscuda_flash_decode": ([P] * 10 + [Z] + [I] * 9 + [F, P], I),
+    "dscuda_flash_cross_forward_workspace_bytes": ([I] * 5, Z),
+    "dscuda_flash_cross_forward": ([P] * 7 + [Z] + [I] * 6 + [F, P], I),
+    "dscuda_flash_cross_backward_workspace_bytes": ([I] * 5, Z),
+    "dscuda_flash_cross_backward": ([P] * 11 + [Z] + [I] * 6 + [F, P], I),
     "dscuda_flash_device_status": ([I], I),
 }
 

@@ -175,7 +175,50 @@ int dscuda_flash_forward(
     int batch, int sequence, int query_heads, int key_value_heads, int dimension,
     float scale, void* stream);
 
-/* No counterpart in the reference: device status of the flash kernel. */
+/* No counterpart in the reference (include/flash_attention.h, flash_rope_cuda).  `sections` is host memory; query or key may be NULL
+ * with its output. */
+int dscuda_flash_rope(
+    void* query_output, void* key_output, const void* query, const void* key, const int* positions,
+    long long rows, int query_heads, int key_heads, int dimension,
+    long long query_output_stride, long long key_output_stride, long long query_stride, long long key_stride,
+    int axes, const int* sections, int restart, int inverse, float theta, void* stream);
+
+/* No counterpart in the reference (flash_cache_append_cuda).  type: 0 int8, 1 e4m3. */
+int dscuda_flash_cache_append(
+    void* key_cache, void* value_cache, float* key_scale, float* value_scale, const void* key, const void* value,
+    const int* block_table, const int* start_positions, const int* token_counts,
+    int batch, int tokens, int key_value_heads, int dimension, long long key_stride, long long value_stride,
+    int page_size, int pages, int cache_blocks, int type, void* stream);
+
+/* No counterpart in the reference (flash_decode_workspace_bytes, flash_decode_cuda). */
+size_t dscuda_flash_decode_workspace_bytes(int tokens, int query_heads, int key_value_heads);
+int dscuda_flash_decode(
+    void* output, float* lse, const void* query, const void* key_cache, const void* value_cache,
+    const float* key_scale, const float* value_scale, const int* block_table, const int* lengths,
+    void* workspace, size_t workspace_bytes,
+    int batch, int tokens, int query_heads, int key_value_heads, int dimension,
+    int page_size, int pages, int cache_blocks, int type, float scale, void* stream);
+
+/* No counterpart in the reference (flash_cross_forward_cuda and its workspace); key_lengths may be NULL. */
+size_t dscuda_flash_cross_forward_workspace_bytes(
+    int batch, int query_length, int key_length, int query_heads, int key_value_heads);
+int dscuda_flash_cross_forward(
+    void* output, float* lse, const void* query, const void* key, const void* value, const int* key_lengths,
+    void* workspace, size_t workspace_bytes,
+    int batch, int query_length, int key_length, int query_heads, int key_value_heads, int dimension,
+    float scale, void* stream);
+
+/* No counterpart in the reference (flash_cross_backward_cuda and its workspace). */
+size_t dscuda_flash_cross_backward_workspace_bytes(
+    int batch, int query_length, int key_length, int query_heads, int key_value_heads);
+int dscuda_flash_cross_backward(
+    void* dquery, void* dkey, void* dvalue, const void* dout, const void* output, const float* lse,
+    const void* query, const void* key, const void* value, const int* key_lengths,
+    void* workspace, size_t workspace_bytes,
+    int batch, int query_length, int key_length, int query_heads, int key_value_heads, int dimension,
+    float scale, void* stream);
+
+/* No counterpart in the reference: device status of the flash kernels (values as for dscuda_mla_device_status). */
 int dscuda_flash_device_status(int reset);
 
 #ifdef __cplusplus
