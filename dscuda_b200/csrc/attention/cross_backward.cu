@@ -7,10 +7,12 @@
 //
 // One call launches:
 //   1. cross_delta_kernel: delta and lse * log2(e) in row order, one pair to a row.
-//   2. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
+//   2. cross_query_kernel: a CTA keeps 128 rows and goes over the keys in tiles of 128: S = Q K^T, dP = dO V^T, dQ += dS K.  With few keys the
+//      rounding of O in delta would be the largest error of dS (2 keys: 0.4 % of dQ and dK, against 0.17 % of the last rounding); where one tile
+//      holds all keys, delta = sum_k P dP is formed from the tile itself and left for the next kernel as well.
+//   3. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
 //      key (two, half the rows each), P^T and dS^T back into tensor memory as bf16 A operands, dV += P^T dO, dK += dS^T Q.  Tensor memory: dV 128, dK
 //      128, two pairs of 64-column scores, so the scores of the next tile are computed while the softmax works on this one.
-//   3. cross_query_kernel: a CTA keeps 128 rows and goes over the keys in tiles of 128: S and dP again, dQ += dS K.
 // S and dP are computed twice (1792 instead of 1280 FLOP per pair).  The alternative of the causal backward, dS stored once and streamed
 // back, moves 4 bytes per pair through HBM, 0.62 ps at the measured copy rate, against 0.31 ps for the 512 FLOP at the measured tensor rate.
 //
@@ -57,7 +59,7 @@ struct CrossBackwardParams {
     CUtensorMap k, v;                   // [B][Tk][Hkv * 128], boxes of 128 rows
     CUtensorMap dq;                     // like q_big
     CUtensorMap dk, dv;                 // like k
-    const float2* rows;                 // [B, Hkv, Tq, group]: lse * log2(e), delta
+    float2* rows;                       // [B, Hkv, Tq, group]: lse * log2(e), delta
     const int* lengths;                 // null: Tk
     int tokens, keys, kv_heads, group;
     int sub_tokens, big_tokens;         // tokens of a query tile of each kind
@@ -439,7 +441,7 @@ constexpr int Q_BYTES = 2 * BIG_CHUNK;
 constexpr int TILE_BYTES = 2 * BIG_CHUNK;
 constexpr int K_SLOTS = 3;
 constexpr int V_SLOTS = 2;                          // the second one first holds dO
-constexpr int MISC_BYTES = 1024;
+constexpr int MISC_BYTES = 2048;
 constexpr int SMEM_BYTES = Q_BYTES + (K_SLOTS + V_SLOTS) * TILE_BYTES + MISC_BYTES + 1024;
 constexpr uint32_t TMEM_S = 0;
 constexpr uint32_t TMEM_DP = 128;
@@ -460,8 +462,10 @@ struct Barriers {
     uint64_t ds_full;
     uint64_t final_full;
     uint64_t staged;
+    uint64_t delta_full;
     uint32_t tmem_base;
     int abort_flag;
+    float delta[2][BIG];        // one key tile: each half's share of sum_k P dP
 };
 static_assert(sizeof(Barriers) <= MISC_BYTES, "barrier block too large");
 }  // namespace queryside
@@ -506,6 +510,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
         mbar_init(smem_u32(&bars->ds_full), SOFTMAX_THREADS);
         mbar_init(smem_u32(&bars->final_full), 1);
         mbar_init(smem_u32(&bars->staged), SOFTMAX_THREADS);
+        mbar_init(smem_u32(&bars->delta_full), SOFTMAX_THREADS);
         bars->abort_flag = 0;
         mbar_init_fence();
     }
@@ -684,11 +689,13 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
         const uint32_t lane_base = static_cast<uint32_t>((warp % 4) * 32) << 16;
         const int token = token0 + r / p.group;
         const bool valid = r < rows_per_tile && token < p.tokens;
+        const size_t row_index = ((static_cast<size_t>(entry) * p.kv_heads + kv_head) * p.tokens + token) * p.group + r % p.group;
         float2 constants = make_float2(INFINITY, 0.0F);
         if (valid) {
-            constants = p.rows[((static_cast<size_t>(entry) * p.kv_heads + kv_head) * p.tokens + token) * p.group + r % p.group];
+            constants = p.rows[row_index];
         }
-        const float lse2 = constants.x, delta = constants.y;
+        const float lse2 = constants.x;
+        float delta = constants.y;
         bool alive = true;
         if (tile_count > 0) {
             alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->resident_full), 0, abort_flag, &cross_backward_status));
@@ -744,6 +751,23 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
             tmem_ld_x32(dp_tmem, sb);
             tmem_ld_x32(dp_tmem + 32, sb + 32);
             tmem_wait_ld();
+            if (tile_count == 1) {
+                float share = 0.0F;
+#pragma unroll
+                for (int n = 0; n < 64; ++n) {
+                    share = fmaf(prob[n], __uint_as_float(sb[n]), share);
+                }
+                bars->delta[half][r] = share;
+                mbar_arrive(smem_u32(&bars->delta_full));
+                alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->delta_full), 0, abort_flag, &cross_backward_status));
+                if (!alive) {
+                    break;
+                }
+                delta = (bars->delta[0][r] + bars->delta[1][r]) / p.scale;
+                if (valid && half == 0) {
+                    p.rows[row_index].y = delta;
+                }
+            }
             uint32_t packed[32];
 #pragma unroll
             for (int n = 0; n < 64; n += 2) {
@@ -859,7 +883,7 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     p.v = make_bf16_batched_tile_map(value, batch_size, key_length, wide, BIG);
     p.dk = make_bf16_batched_tile_map(key_gradient, batch_size, key_length, wide, BIG);
     p.dv = make_bf16_batched_tile_map(value_gradient, batch_size, key_length, wide, BIG);
-    p.rows = static_cast<const float2*>(workspace);
+    p.rows = static_cast<float2*>(workspace);
     p.lengths = key_lengths;
     p.tokens = query_length;
     p.keys = key_length;
@@ -871,9 +895,9 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     const unsigned blocks = static_cast<unsigned>(std::min((rows + 15) / 16, 148LL * 16));
     launch_chained(cross_delta_kernel, dim3(blocks), dim3(256), 0, stream, static_cast<float2*>(workspace), output_gradient, output, logsumexp, rows,
                    query_length, query_heads, p.group);
-    launch_chained(cross_key_kernel, dim3((key_length + BIG - 1) / BIG, key_value_heads, batch_size), dim3(THREADS), keyside::SMEM_BYTES, stream, p);
     launch_chained(cross_query_kernel, dim3((query_length + p.big_tokens - 1) / p.big_tokens, key_value_heads, batch_size), dim3(THREADS),
                    queryside::SMEM_BYTES, stream, p);
+    launch_chained(cross_key_kernel, dim3((key_length + BIG - 1) / BIG, key_value_heads, batch_size), dim3(THREADS), keyside::SMEM_BYTES, stream, p);
 }
 
 }  // namespace dscuda

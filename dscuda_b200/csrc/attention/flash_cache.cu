@@ -2,7 +2,7 @@
 // one fp32 scale for each page and head.
 //
 // A page's scale covers all values that the page holds.  For the new values x of a page and head
-//     need  = max|x| / Q                 (Q = 127 or 448; 0 if max|x| < 2^-100)
+//     need  = max|x| * (1 / Q)           (Q = 127 or 448, 1 / Q as an fp32 constant; 0 if max|x| < 2^-100)
 //     scale = max(old, need)             (old = 0 for a page that starts with a new token)
 //     code  = round(x * (1 / scale))
 // and where the scale grows, the page's older codes become round(code * (old * (1 / scale))).  Every step is a single fp32 operation,
@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(THREADS) flash_cache_append_kernel(const __gri
     for (int w = 0; w < THREADS / 32; ++w) {
         largest = fmaxf(largest, warp_max[w]);
     }
-    const float need = largest < SMALLEST ? 0.0F : __fdiv_rn(largest, LARGEST);
+    const float need = largest < SMALLEST ? 0.0F : __fmul_rn(largest, 1.0F / LARGEST);
     const float scale = fmaxf(old, need);
     const float inverse = scale > 0.0F ? __fdiv_rn(1.0F, scale) : 0.0F;
 

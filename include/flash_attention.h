@@ -73,7 +73,7 @@ constexpr int FLASH_DECODE_MAX_TOKENS = 64;
 // Writes new tokens.  Token t of sequence b goes to position start_positions[b] + t (0 when null), page
 // block_table[b][position / page_size]; token_counts [B] (or null): sequence b appends only its first token_counts[b] of the T rows.
 // key, value [B,T,Hkv,128], a token's heads contiguous, tokens `*_stride` elements apart (entries T * stride).
-// A page's scale covers the values it holds: need = max|new| / 127 (448), or 0 when that maximum is below 2^-100; a page that starts
+// A page's scale covers the values it holds: need = max|new| * (1/127 or 1/448 as FP32), or 0 when that maximum is below 2^-100; a page that starts
 // with a new token takes `need`, another max(its scale, need), and where that raises the scale its older codes are rounded again to
 // the new one.  code = round-half-even(x * (1 / scale)).  NaN becomes 0, an infinity the largest code; neither counts for the scale.
 // A page must not be written for two sequences in one call.  A position or page number outside the cache is not written and

@@ -58,7 +58,7 @@ def append(cache, scales, rows, table, starts, counts):
             for h in range(heads):
                 x = torch.nan_to_num(rows[b, begin - start:end - start, h].float(), nan=0.0, posinf=math.inf, neginf=-math.inf)
                 amax = torch.where(torch.isfinite(x), x.abs(), torch.zeros_like(x)).amax()
-                need = amax / LARGEST[dtype] if amax >= 2.0 ** -100 else torch.tensor(0.0)
+                need = amax * torch.tensor(1.0 / LARGEST[dtype]) if amax >= 2.0 ** -100 else torch.tensor(0.0)
                 old = scales[at, h].clone() if slot > 0 else torch.tensor(0.0)
                 new = torch.maximum(old, need)
                 if new > old and slot > 0:
