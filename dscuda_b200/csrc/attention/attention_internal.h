@@ -35,7 +35,7 @@ void check_flash_cache_shape(int batch_size, int tokens, int key_value_heads, in
 void check_flash_cross_shape(int batch_size, int query_length, int key_length, int query_heads, int key_value_heads, int head_size, float scale);
 
 // Cross attention of few query rows to a key head (group * tokens) on the kernels of flash_decode.cu, and its workspace.
-std::size_t few_rows_workspace_bytes(long long rows);
+std::size_t few_rows_workspace_bytes(int batch, int key_value_heads, long long rows);
 void launch_few_rows_cross(__nv_bfloat16* output, float* logsumexp, const __nv_bfloat16* query, const __nv_bfloat16* key, const __nv_bfloat16* value,
                            const int* key_lengths, void* workspace, int batch, int tokens, int keys, int query_heads, int key_value_heads, float scale,
                            cudaStream_t stream);

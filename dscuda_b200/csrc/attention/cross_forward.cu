@@ -495,7 +495,7 @@ std::size_t flash_cross_forward_workspace_bytes(int batch_size, int query_length
         return 0;
     }
     const long long rows = static_cast<long long>(query_length) * (query_heads / key_value_heads);
-    return rows <= FEW_ROWS ? internal::few_rows_workspace_bytes(rows) : 0;
+    return rows <= FEW_ROWS ? internal::few_rows_workspace_bytes(batch_size, key_value_heads, rows) : 0;
 }
 
 void flash_cross_forward_cuda(__nv_bfloat16* output, float* logsumexp, const __nv_bfloat16* query, const __nv_bfloat16* key,

@@ -13,18 +13,21 @@
 // 128 rows and the widened tile written back to shared memory.
 //
 // Operands.  Codes become f16 (exact for both types: int8 through 1024 + u - 1152, e4m3 by conversion) and so does Q, each row
-// multiplied by a power of two that brings its largest element to 2^13..2^14; P is rounded to f16 (half a step is 2^-12 of it), relative to the largest
-// value scale met so far and times 2^14, so that small weights of long rows keep their bits.  bf16 states are multiplied as they are, P
-// rounded to bf16.  Sums, maxima and the softmax are fp32.
+// multiplied by a power of two that brings its largest element to 2^13..2^14; P is rounded to f16 (half a step is 2^-11 of it), relative to the
+// largest value scale met so far and times 2^14, so that small weights of long rows keep their bits.  bf16 states are multiplied as they
+// are, P rounded to bf16.  Sums, maxima and the softmax are fp32.
 //
-// The order of head columns inside a product is free as long as both factors agree, so a thread takes 16 consecutive bytes of a
-// key (four k-steps of its fragment) instead of a gather, and of a value 16 consecutive bytes of four keys.  Rows in shared memory are
+// Products.  S^T = K Q^T and O^T = V^T P^T: the keys, and then the head columns, are the 16 rows of an instruction, the query rows its 8
+// columns, so that 1 to 8 query rows waste nothing (with the rows on the 16-row side a step of four heads took twice the tensor instructions and
+// twice the softmax: 74 us for 32 ragged sequences where this form takes FIGURE).  The 8 x 8 blocks of P^T are turned by movmatrix.
+// The order of head columns inside a product is free as long as both factors agree, so a thread takes 16 consecutive bytes of a key
+// (four k-steps of its fragment) instead of a gather, and of a value 16 consecutive bytes of four keys.  Rows in shared memory are
 // swizzled by ((r & 7) >> 1) | ((r & 1) << 2) in 16-byte units, which makes both read patterns free of bank conflicts.
 //
 // Work split: tiles of 4 warps x 32 (16) keys of all (sequence, head, row block) items laid end to end and cut into equal ranges, one
 // per CTA.  A warp streams its own keys through its own ring (cp.async, no barriers between warps); the four merge at the end of an
-// item.  An item that one CTA sees whole is written at once, parts go to the workspace and flash_decode_combine_kernel joins
-// them.  No atomics: results do not depend on the order in which CTAs run.
+// item.  An item that one CTA sees whole is written at once, parts go to the workspace, and the CTA with an item's first tile leaves a
+// note of who holds them; flash_decode_combine_kernel joins them.  No atomics: results do not depend on the order in which CTAs run.
 #include "flash_attention.h"
 #include "cuda_common.h"
 #include "attention_internal.h"
@@ -44,10 +47,11 @@ namespace {
 using sm100::exp2_approx;
 
 constexpr int HEAD = 128;
+constexpr int KSTEPS = HEAD / 16;
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int STAGES = 3;
-constexpr int CTAS = 2 * 148;               // two to an SM
+constexpr int MOST_CTAS = 3 * 148;
+constexpr int MERGE_PITCH = HEAD + 4;       // floats between rows of the merge buffer
 constexpr float LOG2E = 1.4426950408889634F;
 constexpr float LN2 = 0.6931471805599453F;
 constexpr float WEIGHT_UNIT = 16384.0F;     // f16 weights are stored times this
@@ -55,6 +59,13 @@ constexpr float WEIGHT_UNIT = 16384.0F;     // f16 weights are stored times this
 enum Source { INT8 = 0, E4M3 = 1, BF16 = 2 };
 
 __device__ int flash_decode_status = 0;
+
+// Who holds the parts of an item: `count` CTAs from `first` on, the first one in its slot 2 * first + `slot`, the others in 2 * cta.
+// count 1: written already.
+struct PartNote {
+    int first;
+    int count_slot;                     // 2 * count + slot
+};
 
 struct DecodeParams {
     const __nv_bfloat16* query;         // [B, T, Hq, 128]
@@ -66,8 +77,9 @@ struct DecodeParams {
     const int* lengths;                 // [B]; null: `keys_most` everywhere
     __nv_bfloat16* out;                 // [B, T, Hq, 128]
     float* lse;                         // [B, Hq, T]
-    float* part_out;                    // [2 * CTAs][rows of a block][128], normalised
-    float* part_lse;                    // [2 * CTAs][rows of a block], log2 domain
+    float* part_out;                    // [2 * MOST_CTAS][rows of a block][128], normalised
+    float* part_lse;                    // [2 * MOST_CTAS][rows of a block], log2 domain
+    PartNote* notes;                    // [B][items]
     int batch, tokens, heads, kv_heads, group;
     int page, pages, blocks;
     int keys_most;                      // pages * page, or Tk
@@ -76,41 +88,56 @@ struct DecodeParams {
     float scale;
 };
 
-template <int SOURCE, int MT>
+// NB: blocks of 8 query rows of an item.
+template <int SOURCE, int NB>
 struct Shape {
+    static constexpr int ROWS = 8 * NB;
     static constexpr int KEYS = SOURCE == BF16 ? 16 : 32;          // of a warp's step
     static constexpr int TILE = WARPS * KEYS;
     static constexpr int ROW_BYTES = SOURCE == BF16 ? 256 : 128;
     static constexpr int OPERAND = KEYS * ROW_BYTES;               // 4 KB
     static constexpr int STAGE = 2 * OPERAND;
-    static constexpr int RING = WARPS * STAGES * STAGE;            // 96 KB
-    static constexpr int ROWS = 16 * MT;
-    static constexpr int QUERY = MT > 1 ? MT * 8 * 512 : 0;        // fragments of Q, when registers do not hold them
-    static constexpr int MERGE = WARPS * ROWS * HEAD * 4;          // in the ring's place, between items
-    static_assert(MERGE <= RING, "merge buffer");
+    static constexpr int CTAS_PER_SM = NB == 1 ? 3 : 2;
+    static constexpr int STAGES = NB == 1 ? 2 : 3;
+    static constexpr int RING = WARPS * STAGES * STAGE;
+    static constexpr int QUERY = NB > 2 ? NB * KSTEPS * 256 : 0;   // fragments of Q, when registers do not hold them
+    static constexpr int MERGE = WARPS * ROWS * MERGE_PITCH * 4;   // in the ring's place, between items
     static constexpr int BYTES = RING + QUERY;
+    static_assert(MERGE <= RING, "merge buffer");
+    static_assert(CTAS_PER_SM * (BYTES + 2048) <= 227 * 1024, "CTAs of an SM");
 };
 
 struct Scales {
     float key[2], value[2];             // of the step's two groups of 16 keys
 };
 
-__device__ __forceinline__ void copy16(uint32_t dst, const void* src, bool valid) {
-    // 16 bytes, or 16 zeros: keys behind the end of a sequence may hold anything
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
+    asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+
+// 16 bytes, or 16 zeros: what lies behind the end of a sequence may be anything
+__device__ __forceinline__ void copy16_if(uint32_t dst, const void* src, bool valid) {
     asm volatile("cp.async.cg.shared.global.L2::128B [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(valid ? 16 : 0) : "memory");
 }
 
 template <int SOURCE>
-__device__ __forceinline__ void mma16816(float (&d)[4], const uint4& a, uint32_t b0, uint32_t b1) {
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], const uint2& b) {
     if constexpr (SOURCE == BF16) {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
     } else {
         asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
             : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-            : "r"(a.x), "r"(a.y), "r"(a.z), "r"(a.w), "r"(b0), "r"(b1));
+            : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b.x), "r"(b.y));
     }
+}
+
+// Turns an 8 x 8 block of 16-bit values: lane (g, c) gives columns 2 c, 2 c + 1 of row g and gets those of the transposed block.
+__device__ __forceinline__ uint32_t turn8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
 }
 
 __device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
@@ -142,282 +169,269 @@ __device__ __forceinline__ uint32_t swizzle(int row) {
     return static_cast<uint32_t>(((row & 7) >> 1) | ((row & 1) << 2));
 }
 
-// Sequences as runs of tiles: entry b has row_blocks * kv_heads items of tiles(b) tiles each.
 __device__ __forceinline__ int length_of(const DecodeParams& p, int b) {
     const int length = p.lengths == nullptr ? p.keys_most : p.lengths[b];
     return min(max(length, 0), p.keys_most);
 }
 
-__device__ __forceinline__ long long tiles_of(const DecodeParams& p, int b, int tile) {
-    return (static_cast<long long>(length_of(p, b)) + tile - 1) / tile;
-}
-
-// Sum of tiles(b) * items over [0, count) by the whole block; every thread gets it.
-__device__ __forceinline__ long long sum_tiles(const DecodeParams& p, int count, int tile, long long* scratch) {
-    long long sum = 0;
-    for (int b = threadIdx.x; b < count; b += THREADS) {
-        sum += tiles_of(p, b, tile);
-    }
-#pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) {
-        sum += __shfl_xor_sync(0xffffffffU, sum, offset);
-    }
-    __syncthreads();
-    if (threadIdx.x % 32 == 0) {
-        scratch[threadIdx.x / 32] = sum;
-    }
-    __syncthreads();
-    sum = 0;
-    for (int w = 0; w < WARPS; ++w) {
-        sum += scratch[w];
-    }
-    return sum * p.kv_heads * p.row_blocks;
-}
-
-__device__ __forceinline__ long long range_start(long long total, int ctas, int cta) {
-    return total * cta / ctas;
-}
-
 // The address of a query or output row: row = token * group + head of the group.
 __device__ __forceinline__ size_t row_offset(const DecodeParams& p, int b, int kv_head, int row) {
     const int token = row / p.group;
-    return ((static_cast<size_t>(b) * p.tokens + token) * p.heads + kv_head * p.group + row % p.group) * HEAD;
+    return ((static_cast<size_t>(b) * p.tokens + token) * p.heads + kv_head * p.group + (row - token * p.group)) * HEAD;
 }
 
 __device__ __forceinline__ size_t lse_offset(const DecodeParams& p, int b, int kv_head, int row) {
-    return (static_cast<size_t>(b) * p.heads + kv_head * p.group + row % p.group) * p.tokens + row / p.group;
+    const int token = row / p.group;
+    return (static_cast<size_t>(b) * p.heads + kv_head * p.group + (row - token * p.group)) * p.tokens + token;
 }
 
-template <int SOURCE, int MT>
-__global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_constant__ DecodeParams p) {
-    using S = Shape<SOURCE, MT>;
+// Equal ranges of tiles: the first total % ctas CTAs take one more than the others.
+struct Ranges {
+    unsigned each, more;
+    __device__ Ranges(unsigned total, unsigned ctas) : each(total / ctas), more(total % ctas) {}
+    __device__ unsigned start(unsigned cta) const { return each * cta + min(cta, more); }
+    __device__ unsigned holder(unsigned tile) const { return tile < (each + 1) * more ? tile / (each + 1) : more + (tile - (each + 1) * more) / each; }
+};
+
+template <int SOURCE, int NB>
+__global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash_decode_kernel(const __grid_constant__ DecodeParams p) {
+    using S = Shape<SOURCE, NB>;
     constexpr int KEYS = S::KEYS;
-    constexpr int NT = KEYS / 8;                        // n-tiles of a step's scores
-    constexpr int KU = KEYS / 16;                       // k-steps of P V
-    constexpr int KSTEPS = HEAD / 16;
+    constexpr int STAGES = S::STAGES;
+    constexpr int KU = KEYS / 16;                       // blocks of 16 keys of a step
+    constexpr bool QUERY_IN_REGISTERS = S::QUERY == 0;
     extern __shared__ __align__(1024) uint8_t smem[];
-    __shared__ long long scratch[WARPS];
     __shared__ Scales scales[WARPS][STAGES];
     __shared__ float merge_m[WARPS][S::ROWS], merge_l[WARPS][S::ROWS], merge_unit[WARPS];
-    __shared__ long long found_first;
-    __shared__ int found_entry;
 
     const int warp = threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
-    const int g = lane / 4;                             // row of a fragment of A and C, column of one of B
+    const int g = lane / 4;
     const int c = lane % 4;
     const uint32_t delta = static_cast<uint32_t>((g >> 1) | ((g & 1) << 2));        // which 16-byte unit of a value row this lane takes
-    const uint32_t ring = warp * STAGES * S::STAGE;             // offset of the warp's ring
+    const uint32_t ring = warp * STAGES * S::STAGE;     // offset of the warp's ring
     const uint32_t smem_base = sm100::smem_u32(smem);
     auto lds128 = [&](uint32_t offset) { return *reinterpret_cast<const uint4*>(smem + offset); };
+    constexpr int LANES = S::ROW_BYTES / 16;            // lanes that copy a row
+    constexpr int COPY_ROWS = 32 / LANES;               // rows of one instruction
+    // rows lane / LANES + COPY_ROWS * i: their place in a stage repeats after 8 rows
+    uint32_t copy_to[8 / COPY_ROWS];
+#pragma unroll
+    for (int i = 0; i < 8 / COPY_ROWS; ++i) {
+        const int row = lane / LANES + COPY_ROWS * i;
+        copy_to[i] = smem_base + ring + row * S::ROW_BYTES + (((lane % LANES) ^ swizzle(row)) * 16);
+    }
 
     sm100::grid_dependency_wait();
-    const long long total = sum_tiles(p, p.batch, S::TILE, scratch);
-    long long position = range_start(total, gridDim.x, blockIdx.x);
-    const long long end = range_start(total, gridDim.x, blockIdx.x + 1);
-    if (position >= end) {
+    // ---- the CTA's range of tiles, and the entry that holds its first one; every warp for itself --------------
+    const unsigned items = p.kv_heads * p.row_blocks;
+    unsigned total = 0;
+    for (int base = 0; base < p.batch; base += 32) {
+        unsigned tiles = base + lane < p.batch ? (length_of(p, base + lane) + S::TILE - 1) / S::TILE * items : 0;
+        total += __reduce_add_sync(0xffffffffU, tiles);
+    }
+    const unsigned ctas = min(total, gridDim.x);        // with a tile each
+    if (blockIdx.x >= ctas) {
         return;
     }
-    // the entry that holds the first tile: blocks of THREADS entries, then inside the block
-    const int items = p.kv_heads * p.row_blocks;
-    long long entry_first = 0;
+    const Ranges ranges(total, ctas);
+    unsigned position = ranges.start(blockIdx.x);
+    const unsigned end = ranges.start(blockIdx.x + 1);
+    unsigned entry_first = 0;
     int entry = 0;
-    {
-        long long before = 0;
-        for (int base = 0; base < p.batch; base += THREADS) {
-            const int b = base + threadIdx.x;
-            const long long own = b < p.batch ? tiles_of(p, b, S::TILE) * items : 0;
-            long long inclusive = own;
+    for (int base = 0;; base += 32) {
+        const unsigned own = base + lane < p.batch ? (length_of(p, base + lane) + S::TILE - 1) / S::TILE * items : 0;
+        unsigned inclusive = own;
 #pragma unroll
-            for (int offset = 1; offset < 32; offset <<= 1) {
-                const long long other = __shfl_up_sync(0xffffffffU, inclusive, offset);
-                if (lane >= offset) {
-                    inclusive += other;
-                }
-            }
-            __syncthreads();
-            if (lane == 31) {
-                scratch[warp] = inclusive;
-            }
-            __syncthreads();
-            long long sum = 0;
-            for (int w = 0; w < WARPS; ++w) {
-                if (w < warp) {
-                    inclusive += scratch[w];
-                }
-                sum += scratch[w];
-            }
-            inclusive += before;
-            if (position >= inclusive - own && position < inclusive) {
-                found_entry = b;
-                found_first = inclusive - own;
-            }
-            before += sum;
-            __syncthreads();
-            if (position < before) {
-                break;
-            }
+        for (int offset = 1; offset < 32; offset <<= 1) {
+            const unsigned other = __shfl_up_sync(0xffffffffU, inclusive, offset);
+            inclusive += lane >= offset ? other : 0;
         }
-        entry = found_entry;
-        entry_first = found_first;
+        const unsigned mine = __ballot_sync(0xffffffffU, position < entry_first + inclusive);
+        if (mine != 0) {
+            const int source = __ffs(mine) - 1;
+            entry = base + source;
+            entry_first += __shfl_sync(0xffffffffU, inclusive - own, source);
+            break;
+        }
+        entry_first += __shfl_sync(0xffffffffU, inclusive, 31);
     }
 
     bool first_segment = true;
     while (position < end) {
         const int length = length_of(p, entry);
-        const long long entry_tiles = tiles_of(p, entry, S::TILE);
+        const unsigned entry_tiles = (length + S::TILE - 1) / S::TILE;
         if (position >= entry_first + entry_tiles * items) {
             entry_first += entry_tiles * items;
             ++entry;
             continue;
         }
-        const long long item = (position - entry_first) / entry_tiles;
-        const long long item_first = entry_first + item * entry_tiles;
+        const unsigned item = (position - entry_first) / entry_tiles;
+        const unsigned item_first = entry_first + item * entry_tiles;
         const int tile_begin = static_cast<int>(position - item_first);
         const int tile_end = static_cast<int>(min(entry_tiles, end - item_first));
-        const int kv_head = static_cast<int>(item / p.row_blocks);
-        const int row_base = static_cast<int>(item % p.row_blocks) * S::ROWS;
+        const int kv_head = static_cast<int>(item) / p.row_blocks;
+        const int row_base = (static_cast<int>(item) - kv_head * p.row_blocks) * S::ROWS;
         const int rows = p.group * p.tokens;
-
-        // ---- Q: fragments in the column order of the codes --------------------------------------------------
-        uint4 qa[MT == 1 ? KSTEPS : 1];
-        float factor[MT][2];            // scale * log2(e) * 2^-shift of the thread's two rows
-        int limit[MT][2];               // keys that they see
-        __syncthreads();                // the last item's merge buffer, and its fragments, have been read
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            uint32_t raw[2][KSTEPS * 2];
-#pragma unroll
-            for (int side = 0; side < 2; ++side) {
-                const int row = row_base + mt * 16 + g + side * 8;
-                limit[mt][side] = row < rows ? (p.causal ? length - p.tokens + 1 + row / p.group : length) : 0;
-                const uint4* src = reinterpret_cast<const uint4*>(p.query + (row < rows ? row_offset(p, entry, kv_head, row) : 0));
-                // 8-bit: k-step 4 j + i holds columns 16 (c + 4 j) + 4 i .. + 3; bf16: k-step 2 j + i columns 8 (c + 4 j) + 4 i .. + 3
-                constexpr int UNITS = 4;
-#pragma unroll
-                for (int u = 0; u < UNITS; ++u) {
-                    const int unit = SOURCE == BF16 ? c + 4 * u : 2 * (c + 4 * (u / 2)) + u % 2;
-                    const uint4 v = row < rows ? src[unit] : make_uint4(0, 0, 0, 0);
-                    raw[side][4 * u] = v.x;
-                    raw[side][4 * u + 1] = v.y;
-                    raw[side][4 * u + 2] = v.z;
-                    raw[side][4 * u + 3] = v.w;
-                }
-                factor[mt][side] = p.scale * LOG2E;
-                if (SOURCE != BF16) {
-                    float largest = 0.0F;
-#pragma unroll
-                    for (int e = 0; e < KSTEPS * 2; ++e) {
-                        largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(raw[side][e] << 16)), fabsf(__uint_as_float(raw[side][e] & 0xffff0000U))));
-                    }
-                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffU, largest, 1));
-                    largest = fmaxf(largest, __shfl_xor_sync(0xffffffffU, largest, 2));
-                    const int exponent = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
-                    const int shift = largest > 0.0F && exponent < 128 ? min(13 - exponent, 120) : 0;
-                    const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
-                    factor[mt][side] *= __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
-#pragma unroll
-                    for (int e = 0; e < KSTEPS * 2; ++e) {
-                        raw[side][e] = pack_f16x2(__uint_as_float(raw[side][e] << 16) * up, __uint_as_float(raw[side][e] & 0xffff0000U) * up);
-                    }
-                }
-            }
-#pragma unroll
-            for (int k = 0; k < KSTEPS; ++k) {
-                const uint4 fragment = make_uint4(raw[0][2 * k], raw[1][2 * k], raw[0][2 * k + 1], raw[1][2 * k + 1]);
-                if constexpr (MT == 1) {
-                    qa[k] = fragment;
-                } else if (warp == mt) {
-                    *reinterpret_cast<uint4*>(smem + S::RING + ((mt * KSTEPS + k) * 32 + lane) * 16) = fragment;
-                }
-            }
-        }
-        if constexpr (MT > 1) {
-            __syncthreads();
-        }
 
         // ---- the warp's keys: steps of KEYS, one to a tile ------------------------------------------------
         const int first_key = tile_begin * S::TILE + warp * KEYS;
         const int steps = min(tile_end - tile_begin, max(0, (length - first_key + S::TILE - 1) / S::TILE));
         uint32_t place[2] = {0, 0};                     // lane l: where step (s / 32) * 32 + l finds its two groups of 16 keys
-        float place_scale[4] = {1.0F, 1.0F, 1.0F, 1.0F};
+        Scales place_scales = {};
         auto issue = [&](int s) {
             if (s < steps) {
-                if (SOURCE != BF16 && s % 32 == 0) {
-                    const int key = first_key + (s + lane) * S::TILE;
-                    if (s + lane < steps) {
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            const int k = min(key + 16 * u, length - 1);
-                            int page = p.table[static_cast<size_t>(entry) * p.pages + k / p.page];
-                            if (page < 0 || page >= p.blocks) {
-                                atomicExch(&flash_decode_status, sm100::STATUS_BAD_INDEX);
-                                page = 0;
-                            }
-                            const uint32_t head_page = static_cast<uint32_t>(page) * p.kv_heads + kv_head;
-                            place[u] = head_page * p.page + (k / 16 * 16) % p.page;
-                            place_scale[u] = p.key_scale[head_page];
-                            place_scale[2 + u] = p.value_scale[head_page];
-                        }
-                    }
-                    __syncwarp();
-                }
-                const uint32_t dst = smem_base + ring + (s % STAGES) * S::STAGE;
                 const int key0 = first_key + s * S::TILE;
+                const uint32_t slot = (s % STAGES) * S::STAGE;
                 if constexpr (SOURCE != BF16) {
-                    uint32_t at[2];
-                    Scales meta;
+                    if (s % 32 == 0) {
+                        const int key = key0 + lane * S::TILE;
+                        if (s + lane < steps) {
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                const int k = min(key + 16 * u, length - 1);
+                                const int logical = k / p.page;
+                                int page = p.table[static_cast<size_t>(entry) * p.pages + logical];
+                                if (page < 0 || page >= p.blocks) {
+                                    atomicExch(&flash_decode_status, sm100::STATUS_BAD_INDEX);
+                                    page = 0;
+                                }
+                                const uint32_t head_page = static_cast<uint32_t>(page) * p.kv_heads + kv_head;
+                                place[u] = head_page * p.page + (k / 16 * 16 - logical * p.page);
+                                place_scales.key[u] = p.key_scale[head_page];
+                                place_scales.value[u] = p.value_scale[head_page];
+                            }
+                        }
+                        __syncwarp();
+                    }
+                    if (lane == s % 32) {
+                        scales[warp][s % STAGES] = place_scales;
+                    }
 #pragma unroll
                     for (int u = 0; u < 2; ++u) {
-                        at[u] = __shfl_sync(0xffffffffU, place[u], s % 32);
-                        meta.key[u] = __shfl_sync(0xffffffffU, place_scale[u], s % 32);
-                        meta.value[u] = __shfl_sync(0xffffffffU, place_scale[2 + u], s % 32);
-                    }
-                    if (lane == 0) {
-                        scales[warp][s % STAGES] = meta;
-                    }
+                        const uint32_t at = __shfl_sync(0xffffffffU, place[u], s % 32);
+                        const size_t offset = static_cast<size_t>(at) * 128 + lane * 16;        // rows of a group lie one after the other
+                        const uint8_t *k = p.keys + offset, *v = p.values + offset;
+                        const int left = length - key0 - 16 * u;
+                        if (left >= 16) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        const int row = lane / 8 + 4 * i;
-                        const bool valid = key0 + row < length;
-                        const size_t offset = valid ? static_cast<size_t>(at[i / 4] + row % 16) * 128 + (lane % 8) * 16 : 0;
-                        const uint32_t to = row * 128 + (((lane % 8) ^ swizzle(row)) * 16);
-                        copy16(dst + to, p.keys + offset, valid);
-                        copy16(dst + S::OPERAND + to, p.values + offset, valid);
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t to = copy_to[i % 2] + slot + (16 * u + 8 * (i / 2)) * 128;
+                                copy16(to, k + i * 512);
+                                copy16(to + S::OPERAND, v + i * 512);
+                            }
+                        } else {
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const uint32_t to = copy_to[i % 2] + slot + (16 * u + 8 * (i / 2)) * 128;
+                                const bool valid = lane / 8 + 4 * i < left;
+                                copy16_if(to, valid ? k + i * 512 : p.keys, valid);
+                                copy16_if(to + S::OPERAND, valid ? v + i * 512 : p.values, valid);
+                            }
+                        }
                     }
                 } else {
+                    const size_t pitch = static_cast<size_t>(p.kv_heads) * 256;
+                    const size_t offset = (static_cast<size_t>(entry) * p.keys_most + key0 + lane / 16) * pitch + kv_head * 256 + (lane % 16) * 16;
+                    const uint8_t *k = p.keys + offset, *v = p.values + offset;
+                    const int left = length - key0;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        const int row = lane / 16 + 2 * i;
-                        const bool valid = key0 + row < length;
-                        const size_t offset = valid ? ((static_cast<size_t>(entry) * p.keys_most + key0 + row) * p.kv_heads + kv_head) * 256 + (lane % 16) * 16 : 0;
-                        const uint32_t to = row * 256 + (((lane % 16) ^ swizzle(row)) * 16);
-                        copy16(dst + to, p.keys + offset, valid);
-                        copy16(dst + S::OPERAND + to, p.values + offset, valid);
+                        const uint32_t to = copy_to[i % 4] + slot + 8 * (i / 4) * 256;
+                        const bool valid = lane / 16 + 2 * i < left;
+                        copy16_if(to, valid ? k + 2 * i * pitch : p.keys, valid);
+                        copy16_if(to + S::OPERAND, valid ? v + 2 * i * pitch : p.values, valid);
                     }
                 }
             }
             asm volatile("cp.async.commit_group;" ::: "memory");
         };
-
-        float o[MT][16][4];
-        float m[MT][2], l[MT][2];
-        float unit = 0.0F;              // the largest value scale so far: weights are relative to it
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-#pragma unroll
-            for (int q = 0; q < 16; ++q) {
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    o[mt][q][e] = 0.0F;
-                }
-            }
-            m[mt][0] = m[mt][1] = -INFINITY;
-            l[mt][0] = l[mt][1] = 0.0F;
-        }
+        __syncthreads();                // the last item's merge buffer has been read
 #pragma unroll
         for (int s = 0; s < STAGES - 1; ++s) {
             issue(s);
+        }
+
+        // ---- Q: B fragments in the column order of the codes; lane (g, c) has row g of each block ----------------
+        uint2 query[QUERY_IN_REGISTERS ? NB : 1][KSTEPS];
+        float factor[NB][2];            // scale * log2(e) * 2^-shift of rows 2 c and 2 c + 1
+        int limit[NB][2];               // keys that they see
+        int least = 0x7fffffff;         // the fewest that a row sees
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int row = row_base + nb * 8 + g;
+            const uint4* src = reinterpret_cast<const uint4*>(p.query + (row < rows ? row_offset(p, entry, kv_head, row) : 0));
+            uint32_t raw[KSTEPS * 2];
+            // 8-bit: k-step 4 j + i holds columns 16 (c + 4 j) + 4 i .. + 3; bf16: k-step 2 j + i columns 8 (c + 4 j) + 4 i .. + 3
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                const int unit = SOURCE == BF16 ? c + 4 * u : 2 * (c + 4 * (u / 2)) + u % 2;
+                const uint4 v = row < rows ? src[unit] : make_uint4(0, 0, 0, 0);
+                raw[4 * u] = v.x;
+                raw[4 * u + 1] = v.y;
+                raw[4 * u + 2] = v.z;
+                raw[4 * u + 3] = v.w;
+            }
+            float down = p.scale * LOG2E;
+            if (SOURCE != BF16) {
+                float largest = 0.0F;
+#pragma unroll
+                for (int e = 0; e < KSTEPS * 2; ++e) {
+                    largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(raw[e] << 16)), fabsf(__uint_as_float(raw[e] & 0xffff0000U))));
+                }
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffU, largest, 1));
+                largest = fmaxf(largest, __shfl_xor_sync(0xffffffffU, largest, 2));
+                const int exponent = static_cast<int>(__float_as_uint(largest) >> 23) - 127;
+                const int shift = largest > 0.0F && exponent < 128 ? min(13 - exponent, 120) : 0;
+                const float up = __uint_as_float(static_cast<uint32_t>(127 + shift) << 23);
+                down *= __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
+#pragma unroll
+                for (int e = 0; e < KSTEPS * 2; ++e) {
+                    raw[e] = pack_f16x2(__uint_as_float(raw[e] << 16) * up, __uint_as_float(raw[e] & 0xffff0000U) * up);
+                }
+            }
+#pragma unroll
+            for (int side = 0; side < 2; ++side) {
+                const int column = row_base + nb * 8 + 2 * c + side;
+                factor[nb][side] = __shfl_sync(0xffffffffU, down, 8 * c + 4 * side);
+                limit[nb][side] = column < rows ? (p.causal ? length - p.tokens + 1 + column / p.group : length) : 0;
+                least = min(least, limit[nb][side]);
+            }
+#pragma unroll
+            for (int k = 0; k < KSTEPS; ++k) {
+                if constexpr (QUERY_IN_REGISTERS) {
+                    query[nb][k] = make_uint2(raw[2 * k], raw[2 * k + 1]);
+                } else if (warp == nb % WARPS) {
+                    *reinterpret_cast<uint2*>(smem + S::RING + ((nb * KSTEPS + k) * 32 + lane) * 8) = make_uint2(raw[2 * k], raw[2 * k + 1]);
+                }
+            }
+        }
+        least = __reduce_min_sync(0xffffffffU, least);
+        if constexpr (!QUERY_IN_REGISTERS) {
+            __syncthreads();
+        }
+        auto query_fragment = [&](int nb, int k) {
+            if constexpr (QUERY_IN_REGISTERS) {
+                return query[nb][k];
+            } else {
+                return *reinterpret_cast<const uint2*>(smem + S::RING + ((nb * KSTEPS + k) * 32 + lane) * 8);
+            }
+        };
+
+        float o[NB][8][4];              // O^T: m-tile j holds head columns 2 j and 2 j + 1 of the lane's unit; query rows 2 c and 2 c + 1
+        float m[NB][2], l[NB][2];
+        float unit = 0.0F;              // the largest value scale so far: weights are relative to it
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    o[nb][j][e] = 0.0F;
+                }
+            }
+            m[nb][0] = m[nb][1] = -INFINITY;
+            l[nb][0] = l[nb][1] = 0.0F;
         }
         for (int s = 0; s < steps; ++s) {
             __syncwarp();               // every lane has read the slot that is filled next
@@ -428,15 +442,15 @@ __global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_c
             const uint32_t values = keys + S::OPERAND;
             const int key0 = first_key + s * S::TILE;
 
-            // S = Q K^T
-            float score[MT][NT][4];
+            // S^T = K Q^T: lane (g, c) gets keys g and g + 8 of a block of 16, query rows 2 c and 2 c + 1
+            float score[KU][NB][4];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
+            for (int u = 0; u < KU; ++u) {
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
+                for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
-                        score[mt][t][e] = 0.0F;
+                        score[u][nb][e] = 0.0F;
                     }
                 }
             }
@@ -444,36 +458,33 @@ __global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_c
             constexpr int STEPS_PER_LOAD = KSTEPS / KLOADS;
 #pragma unroll
             for (int j = 0; j < KLOADS; ++j) {
-                uint4 words[NT];
+                uint4 words[KU][2];
 #pragma unroll
-                for (int t = 0; t < NT; ++t) {
-                    words[t] = lds128(keys + (8 * t + g) * S::ROW_BYTES + (((c + 4 * j) ^ swizzle(g)) * 16));
+                for (int u = 0; u < KU; ++u) {
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        words[u][h] = lds128(keys + (16 * u + 8 * h + g) * S::ROW_BYTES + (((c + 4 * j) ^ swizzle(g)) * 16));
+                    }
                 }
 #pragma unroll
                 for (int i = 0; i < STEPS_PER_LOAD; ++i) {
                     const int k = j * STEPS_PER_LOAD + i;
-                    uint4 a[MT];
 #pragma unroll
-                    for (int mt = 0; mt < MT; ++mt) {
-                        if constexpr (MT == 1) {
-                            a[mt] = qa[k];
-                        } else {
-                            a[mt] = lds128(S::RING + ((mt * KSTEPS + k) * 32 + lane) * 16);
-                        }
-                    }
-#pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const uint32_t* w = reinterpret_cast<const uint32_t*>(&words[t]);
-                        uint32_t b0, b1;
+                    for (int u = 0; u < KU; ++u) {
+                        const uint32_t *w0 = reinterpret_cast<const uint32_t*>(&words[u][0]), *w1 = reinterpret_cast<const uint32_t*>(&words[u][1]);
+                        uint32_t a[4];
                         if constexpr (SOURCE == BF16) {
-                            b0 = w[2 * i];
-                            b1 = w[2 * i + 1];
+                            a[0] = w0[2 * i];
+                            a[1] = w1[2 * i];
+                            a[2] = w0[2 * i + 1];
+                            a[3] = w1[2 * i + 1];
                         } else {
-                            widen<SOURCE>(w[i], b0, b1);
+                            widen<SOURCE>(w0[i], a[0], a[2]);
+                            widen<SOURCE>(w1[i], a[1], a[3]);
                         }
 #pragma unroll
-                        for (int mt = 0; mt < MT; ++mt) {
-                            mma16816<SOURCE>(score[mt][t], a[mt], b0, b1);
+                        for (int nb = 0; nb < NB; ++nb) {
+                            mma16816<SOURCE>(score[u][nb], a, query_fragment(nb, k));
                         }
                     }
                 }
@@ -492,72 +503,76 @@ __global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_c
                     shrink = unit / largest;
                     unit = largest;
                 }
-                const float inverse = unit > 0.0F ? WEIGHT_UNIT / unit : 0.0F;
+                const float inverse = unit > 0.0F ? __fdividef(WEIGHT_UNIT, unit) : 0.0F;
 #pragma unroll
                 for (int u = 0; u < KU; ++u) {
                     key_scale[u] = meta.key[u];
                     value_scale[u] = meta.value[u] * inverse;
                 }
             }
-            uint4 weights[MT][KU];
+            const bool masked = key0 + KEYS > least;
+            uint2 weights[KU][NB];
+            bool moved = shrink != 1.0F;
+            float alpha[NB][2];
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                float alpha[2];
+            for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                 for (int side = 0; side < 2; ++side) {
                     float top = -INFINITY;
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
-                        const float f = factor[mt][side] * key_scale[t / 2];
-#pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float x = score[mt][t][2 * side + e] * f;
-                            score[mt][t][2 * side + e] = key0 + 8 * t + 2 * c + e < limit[mt][side] ? x : -INFINITY;
-                            top = fmaxf(top, score[mt][t][2 * side + e]);
+                    for (int u = 0; u < KU; ++u) {
+                        const float f = factor[nb][side] * key_scale[u];
+                        score[u][nb][side] *= f;
+                        score[u][nb][2 + side] *= f;
+                        if (masked) {
+                            score[u][nb][side] = key0 + 16 * u + g < limit[nb][side] ? score[u][nb][side] : -INFINITY;
+                            score[u][nb][2 + side] = key0 + 16 * u + 8 + g < limit[nb][side] ? score[u][nb][2 + side] : -INFINITY;
                         }
+                        top = sm100::max3(top, score[u][nb][side], score[u][nb][2 + side]);
                     }
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 1));
-                    top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, 2));
-                    const float now = fmaxf(m[mt][side], top);
+#pragma unroll
+                    for (int offset = 4; offset < 32; offset <<= 1) {
+                        top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, offset));
+                    }
+                    const float now = fmaxf(m[nb][side], top);
                     const float reference = now == -INFINITY ? 0.0F : now;          // no key so far: all weights are exp2(-inf) = 0
-                    alpha[side] = exp2_approx(m[mt][side] - reference);
-                    m[mt][side] = now;
+                    alpha[nb][side] = exp2_approx(m[nb][side] - reference);
+                    m[nb][side] = now;
                     float sum = 0.0F;
 #pragma unroll
-                    for (int t = 0; t < NT; ++t) {
+                    for (int u = 0; u < KU; ++u) {
 #pragma unroll
-                        for (int e = 0; e < 2; ++e) {
-                            const float weight = exp2_approx(score[mt][t][2 * side + e] - reference);
+                        for (int h = 0; h < 2; ++h) {
+                            const float weight = exp2_approx(score[u][nb][2 * h + side] - reference);
                             sum += weight;
-                            score[mt][t][2 * side + e] = SOURCE == BF16 ? weight : weight * value_scale[t / 2];
+                            score[u][nb][2 * h + side] = SOURCE == BF16 ? weight : weight * value_scale[u];
                         }
                     }
-                    l[mt][side] = l[mt][side] * alpha[side] + sum;
-                    alpha[side] *= shrink;
-                }
-                if (__any_sync(0xffffffffU, alpha[0] != 1.0F || alpha[1] != 1.0F)) {
-#pragma unroll
-                    for (int q = 0; q < 16; ++q) {
-                        o[mt][q][0] *= alpha[0];
-                        o[mt][q][1] *= alpha[0];
-                        o[mt][q][2] *= alpha[1];
-                        o[mt][q][3] *= alpha[1];
-                    }
+                    l[nb][side] = l[nb][side] * alpha[nb][side] + sum;
+                    alpha[nb][side] *= shrink;
+                    moved |= alpha[nb][side] != 1.0F;
                 }
 #pragma unroll
                 for (int u = 0; u < KU; ++u) {
-                    const float(&x)[4] = score[mt][2 * u];
-                    const float(&y)[4] = score[mt][2 * u + 1];
-                    if constexpr (SOURCE == BF16) {
-                        weights[mt][u] = make_uint4(sm100::pack_bf16x2(x[0], x[1]), sm100::pack_bf16x2(x[2], x[3]), sm100::pack_bf16x2(y[0], y[1]),
-                                                    sm100::pack_bf16x2(y[2], y[3]));
-                    } else {
-                        weights[mt][u] = make_uint4(pack_f16x2(x[0], x[1]), pack_f16x2(x[2], x[3]), pack_f16x2(y[0], y[1]), pack_f16x2(y[2], y[3]));
+                    const float(&x)[4] = score[u][nb];
+                    weights[u][nb].x = turn8x8(SOURCE == BF16 ? sm100::pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]));
+                    weights[u][nb].y = turn8x8(SOURCE == BF16 ? sm100::pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]));
+                }
+            }
+            if (__any_sync(0xffffffffU, moved)) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) {
+                        o[nb][j][0] *= alpha[nb][0];
+                        o[nb][j][1] *= alpha[nb][1];
+                        o[nb][j][2] *= alpha[nb][0];
+                        o[nb][j][3] *= alpha[nb][1];
                     }
                 }
             }
 
-            // O += P V
+            // O^T += V^T P^T
 #pragma unroll
             for (int u = 0; u < KU; ++u) {
                 constexpr int VLOADS = S::ROW_BYTES / 128;
@@ -569,33 +584,27 @@ __global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_c
                         const int row = 16 * u + 8 * (e / 2) + 2 * c + e % 2;
                         rows4[e] = lds128(values + row * S::ROW_BYTES + (((delta + 8 * h) ^ swizzle(row)) * 16));
                     }
-                    const uint32_t* w0 = reinterpret_cast<const uint32_t*>(&rows4[0]);
-                    const uint32_t* w1 = reinterpret_cast<const uint32_t*>(&rows4[1]);
-                    const uint32_t* w2 = reinterpret_cast<const uint32_t*>(&rows4[2]);
-                    const uint32_t* w3 = reinterpret_cast<const uint32_t*>(&rows4[3]);
+                    const uint32_t *w0 = reinterpret_cast<const uint32_t*>(&rows4[0]), *w1 = reinterpret_cast<const uint32_t*>(&rows4[1]);
+                    const uint32_t *w2 = reinterpret_cast<const uint32_t*>(&rows4[2]), *w3 = reinterpret_cast<const uint32_t*>(&rows4[3]);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if constexpr (SOURCE == BF16) {
+                            const uint32_t a[4] = {__byte_perm(w0[i], w1[i], 0x5410), __byte_perm(w0[i], w1[i], 0x7632), __byte_perm(w2[i], w3[i], 0x5410),
+                                                   __byte_perm(w2[i], w3[i], 0x7632)};
 #pragma unroll
-                            for (int e = 0; e < 2; ++e) {
-                                const uint32_t b0 = __byte_perm(w0[i], w1[i], e == 0 ? 0x5410 : 0x7632);
-                                const uint32_t b1 = __byte_perm(w2[i], w3[i], e == 0 ? 0x5410 : 0x7632);
-#pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) {
-                                    mma16816<SOURCE>(o[mt][8 * h + 2 * i + e], weights[mt][u], b0, b1);
-                                }
+                            for (int nb = 0; nb < NB; ++nb) {
+                                mma16816<SOURCE>(o[nb][4 * h + i], a, weights[u][nb]);
                             }
                         } else {
-                            uint32_t b0[4], b1[4];
-                            widen<SOURCE>(__byte_perm(w0[i], w1[i], 0x5140), b0[0], b0[1]);
-                            widen<SOURCE>(__byte_perm(w0[i], w1[i], 0x7362), b0[2], b0[3]);
-                            widen<SOURCE>(__byte_perm(w2[i], w3[i], 0x5140), b1[0], b1[1]);
-                            widen<SOURCE>(__byte_perm(w2[i], w3[i], 0x7362), b1[2], b1[3]);
 #pragma unroll
-                            for (int e = 0; e < 4; ++e) {
+                            for (int e = 0; e < 2; ++e) {
+                                // columns 4 i + 2 e and + 1 of four keys
+                                uint32_t a[4];
+                                widen<SOURCE>(__byte_perm(w0[i], w1[i], e == 0 ? 0x5140 : 0x7362), a[0], a[1]);
+                                widen<SOURCE>(__byte_perm(w2[i], w3[i], e == 0 ? 0x5140 : 0x7362), a[2], a[3]);
 #pragma unroll
-                                for (int mt = 0; mt < MT; ++mt) {
-                                    mma16816<SOURCE>(o[mt][4 * i + e], weights[mt][u], b0[e], b1[e]);
+                                for (int nb = 0; nb < NB; ++nb) {
+                                    mma16816<SOURCE>(o[nb][2 * i + e], a, weights[u][nb]);
                                 }
                             }
                         }
@@ -609,28 +618,24 @@ __global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_c
         __syncthreads();                // every ring is idle: the merge buffer takes its place
         float* merge = reinterpret_cast<float*>(smem);
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
+        for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
             for (int side = 0; side < 2; ++side) {
-                float sum = l[mt][side];
-                sum += __shfl_xor_sync(0xffffffffU, sum, 1);
-                sum += __shfl_xor_sync(0xffffffffU, sum, 2);
-                const int row = mt * 16 + g + side * 8;
-                if (c == 0) {
-                    merge_m[warp][row] = m[mt][side];
+                float sum = l[nb][side];
+#pragma unroll
+                for (int offset = 4; offset < 32; offset <<= 1) {
+                    sum += __shfl_xor_sync(0xffffffffU, sum, offset);
+                }
+                const int row = nb * 8 + 2 * c + side;
+                if (g == 0) {
+                    merge_m[warp][row] = m[nb][side];
                     merge_l[warp][row] = sum;
                 }
-                float* dst = merge + (warp * S::ROWS + row) * HEAD;
-                // column e of n-tile q is head column 16 delta(e) + q (8 bits), 8 (delta(e) + 8 (q / 8)) + q % 8 (bf16); delta(2 c) = c, delta(2 c + 1) = c + 4
+                float* dst = merge + (warp * S::ROWS + row) * MERGE_PITCH;
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int d = c + 4 * e;
-#pragma unroll
-                    for (int q = 0; q < 16; q += 4) {
-                        const int column = SOURCE == BF16 ? 8 * (d + 8 * (q / 8)) + q % 8 : 16 * d + q;
-                        *reinterpret_cast<float4*>(dst + column) =
-                            make_float4(o[mt][q][2 * side + e], o[mt][q + 1][2 * side + e], o[mt][q + 2][2 * side + e], o[mt][q + 3][2 * side + e]);
-                    }
+                for (int j = 0; j < 8; j += 2) {
+                    const int column = SOURCE == BF16 ? 8 * (delta + 8 * (j / 4)) + 2 * (j % 4) : 16 * delta + 2 * j;
+                    *reinterpret_cast<float4*>(dst + column) = make_float4(o[nb][j][side], o[nb][j][2 + side], o[nb][j + 1][side], o[nb][j + 1][2 + side]);
                 }
             }
         }
@@ -638,12 +643,16 @@ __global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_c
             merge_unit[warp] = SOURCE == BF16 ? 1.0F : unit / WEIGHT_UNIT;
         }
         __syncthreads();
-        const bool whole = tile_begin == 0 && tile_end == entry_tiles;
-        const int slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
-        constexpr int PER_ROW = THREADS / 16;           // threads to a row
+        const bool whole = tile_begin == 0 && tile_end == static_cast<int>(entry_tiles);
+        const unsigned slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
+        if (tile_begin == 0 && threadIdx.x == 0) {
+            const int holders = static_cast<int>(ranges.holder(item_first + entry_tiles - 1) - blockIdx.x) + 1;
+            p.notes[static_cast<size_t>(entry) * items + item] = {static_cast<int>(blockIdx.x), 2 * holders + (first_segment ? 0 : 1)};
+        }
+        constexpr int PER_ROW = THREADS / 8;            // threads to a row
 #pragma unroll
-        for (int pass = 0; pass < MT; ++pass) {
-            const int row = pass * 16 + threadIdx.x / PER_ROW;
+        for (int pass = 0; pass < NB; ++pass) {
+            const int row = pass * 8 + threadIdx.x / PER_ROW;
             float top = -INFINITY;
 #pragma unroll
             for (int w = 0; w < WARPS; ++w) {
@@ -660,30 +669,33 @@ __global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_c
             const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
             const float lse2 = sum == 0.0F ? -INFINITY : reference + log2f(sum);
             const int absolute = row_base + row;
-            if (whole && absolute < rows && threadIdx.x % PER_ROW == 0) {
-                p.lse[lse_offset(p, entry, kv_head, absolute)] = lse2 * LN2;
-            }
-            if (!whole && threadIdx.x % PER_ROW == 0) {
-                p.part_lse[static_cast<size_t>(slot) * S::ROWS + row] = lse2;
-            }
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                const int column = ((k * PER_ROW) + threadIdx.x % PER_ROW) * 4;
-                float4 sum4 = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-#pragma unroll
-                for (int w = 0; w < WARPS; ++w) {
-                    const float4 x = *reinterpret_cast<const float4*>(merge + (w * S::ROWS + row) * HEAD + column);
-                    sum4.x += x.x * share[w];
-                    sum4.y += x.y * share[w];
-                    sum4.z += x.z * share[w];
-                    sum4.w += x.w * share[w];
+            if (absolute < rows) {
+                if (threadIdx.x % PER_ROW == 0) {
+                    if (whole) {
+                        p.lse[lse_offset(p, entry, kv_head, absolute)] = lse2 * LN2;
+                    } else {
+                        p.part_lse[static_cast<size_t>(slot) * S::ROWS + row] = lse2;
+                    }
                 }
-                sum4 = make_float4(sum4.x * inverse, sum4.y * inverse, sum4.z * inverse, sum4.w * inverse);
-                if (!whole) {
-                    *reinterpret_cast<float4*>(p.part_out + (static_cast<size_t>(slot) * S::ROWS + row) * HEAD + column) = sum4;
-                } else if (absolute < rows) {
-                    *reinterpret_cast<uint2*>(p.out + row_offset(p, entry, kv_head, absolute) + column) =
-                        make_uint2(sm100::pack_bf16x2(sum4.x, sum4.y), sm100::pack_bf16x2(sum4.z, sum4.w));
+                const size_t out_row = row_offset(p, entry, kv_head, absolute);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const int column = ((k * PER_ROW) + threadIdx.x % PER_ROW) * 4;
+                    float4 sum4 = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+#pragma unroll
+                    for (int w = 0; w < WARPS; ++w) {
+                        const float4 x = *reinterpret_cast<const float4*>(merge + (w * S::ROWS + row) * MERGE_PITCH + column);
+                        sum4.x += x.x * share[w];
+                        sum4.y += x.y * share[w];
+                        sum4.z += x.z * share[w];
+                        sum4.w += x.w * share[w];
+                    }
+                    sum4 = make_float4(sum4.x * inverse, sum4.y * inverse, sum4.z * inverse, sum4.w * inverse);
+                    if (whole) {
+                        *reinterpret_cast<uint2*>(p.out + out_row + column) = make_uint2(sm100::pack_bf16x2(sum4.x, sum4.y), sm100::pack_bf16x2(sum4.z, sum4.w));
+                    } else {
+                        *reinterpret_cast<float4*>(p.part_out + (static_cast<size_t>(slot) * S::ROWS + row) * HEAD + column) = sum4;
+                    }
                 }
             }
         }
@@ -692,92 +704,107 @@ __global__ void __launch_bounds__(THREADS, 2) flash_decode_kernel(const __grid_c
     }
 }
 
-// Joins the parts of the items that several CTAs worked on, in the order of their keys, and writes the rows of entries without any key.
-// A block takes one row of one item.
-__global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __grid_constant__ DecodeParams p, int tile, int block_rows, int ctas) {
-    __shared__ long long scratch[WARPS];
+// Joins the parts of the items that several CTAs worked on, in the order of their keys, and writes the rows of entries without any key.  A
+// warp takes a row, a lane four of its columns.
+__global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __grid_constant__ DecodeParams p, int block_rows) {
     const int rows = p.group * p.tokens;
+    const int index = blockIdx.x * WARPS + threadIdx.x / 32;        // kv_head * rows + row
+    const int lane = threadIdx.x % 32;
     const int entry = blockIdx.y;
-    const int kv_head = blockIdx.x / rows;
-    const int row = blockIdx.x % rows;
-    const int item = kv_head * p.row_blocks + row / block_rows;
+    if (index >= p.kv_heads * rows) {
+        return;
+    }
+    const int kv_head = index / rows;
+    const int row = index - kv_head * rows;
+    const int block = row / block_rows;
     sm100::grid_dependency_wait();
-    const long long tiles = tiles_of(p, entry, tile);
-    __nv_bfloat16* out = p.out + row_offset(p, entry, kv_head, row);
-    if (tiles == 0) {
-        out[threadIdx.x] = __float2bfloat16(0.0F);
-        if (threadIdx.x == 0) {
-            p.lse[lse_offset(p, entry, kv_head, row)] = -INFINITY;
+    const int length = length_of(p, entry);
+    const PartNote note = p.notes[(static_cast<size_t>(entry) * p.kv_heads + kv_head) * p.row_blocks + block];
+    uint2* out = reinterpret_cast<uint2*>(p.out + row_offset(p, entry, kv_head, row)) + lane;
+    float* lse = p.lse + lse_offset(p, entry, kv_head, row);
+    if (length == 0) {
+        *out = make_uint2(0, 0);
+        if (lane == 0) {
+            *lse = -INFINITY;
         }
         return;
     }
-    const long long total = sum_tiles(p, p.batch, tile, scratch);
-    const long long first = sum_tiles(p, entry, tile, scratch) + item * tiles;
-    // the CTA whose range holds a tile: the last one that starts at or before it
-    auto holder = [&](long long at) {
-        int cta = static_cast<int>(at * ctas / total);
-        while (cta + 1 < ctas && range_start(total, ctas, cta + 1) <= at) {
-            ++cta;
-        }
-        while (range_start(total, ctas, cta) > at) {
-            --cta;
-        }
-        return cta;
-    };
-    const int cta_first = holder(first), cta_last = holder(first + tiles - 1);
-    if (cta_first == cta_last) {
-        return;                         // written by that CTA
+    const int count = note.count_slot / 2;
+    if (count <= 1) {
+        return;                         // written by the CTA that saw all of it
     }
-    auto slot_of = [&](int cta) { return 2 * cta + (range_start(total, ctas, cta) >= first ? 0 : 1); };
-    const int inside = row % block_rows;
+    const int inside = row - block * block_rows;
+    auto slot_row = [&](int part) {
+        return static_cast<size_t>(2 * (note.first + part) + (part == 0 ? note.count_slot % 2 : 0)) * block_rows + inside;
+    };
     float top = -INFINITY;
-    for (int cta = cta_first; cta <= cta_last; ++cta) {
-        if (range_start(total, ctas, cta) < range_start(total, ctas, cta + 1)) {
-            top = fmaxf(top, p.part_lse[static_cast<size_t>(slot_of(cta)) * block_rows + inside]);
-        }
+    for (int part = lane; part < count; part += 32) {
+        top = fmaxf(top, p.part_lse[slot_row(part)]);
+    }
+#pragma unroll
+    for (int offset = 16; offset > 0; offset >>= 1) {
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, offset));
     }
     const float reference = top == -INFINITY ? 0.0F : top;
-    float sum = 0.0F, value = 0.0F;
-    for (int cta = cta_first; cta <= cta_last; ++cta) {
-        if (range_start(total, ctas, cta) < range_start(total, ctas, cta + 1)) {
-            const size_t slot = static_cast<size_t>(slot_of(cta)) * block_rows + inside;
-            const float weight = exp2_approx(p.part_lse[slot] - reference);
-            sum += weight;
-            value += weight * p.part_out[slot * HEAD + threadIdx.x];
-        }
+    float sum = 0.0F;
+    float4 value = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+#pragma unroll 4
+    for (int part = 0; part < count; ++part) {
+        const size_t at = slot_row(part);
+        const float weight = exp2_approx(p.part_lse[at] - reference);
+        const float4 x = *reinterpret_cast<const float4*>(p.part_out + at * HEAD + lane * 4);
+        sum += weight;
+        value.x += weight * x.x;
+        value.y += weight * x.y;
+        value.z += weight * x.z;
+        value.w += weight * x.w;
     }
-    out[threadIdx.x] = __float2bfloat16(sum == 0.0F ? 0.0F : value / sum);
-    if (threadIdx.x == 0) {
-        p.lse[lse_offset(p, entry, kv_head, row)] = sum == 0.0F ? -INFINITY : (reference + log2f(sum)) * LN2;
+    const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
+    *out = make_uint2(sm100::pack_bf16x2(value.x * inverse, value.y * inverse), sm100::pack_bf16x2(value.z * inverse, value.w * inverse));
+    if (lane == 0) {
+        *lse = sum == 0.0F ? -INFINITY : (reference + log2f(sum)) * LN2;
     }
 }
 
-template <int SOURCE, int MT>
+// Blocks of 8 query rows that an item has.
+int blocks_of_rows(long long rows) {
+    return rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+}
+
+template <int SOURCE, int NB>
 void launch_decode(DecodeParams& p, cudaStream_t stream) {
-    using S = Shape<SOURCE, MT>;
+    using S = Shape<SOURCE, NB>;
     static bool done[16] = {};
     int device = 0;
     CUDA_CHECK(cudaGetDevice(&device));
     if (device >= 16 || !done[device]) {
-        CUDA_CHECK(cudaFuncSetAttribute(flash_decode_kernel<SOURCE, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+        CUDA_CHECK(cudaFuncSetAttribute(flash_decode_kernel<SOURCE, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
         if (device < 16) {
             done[device] = true;
         }
     }
-    p.row_blocks = (p.group * p.tokens + S::ROWS - 1) / S::ROWS;
+    const int rows = p.group * p.tokens;
+    p.row_blocks = (rows + S::ROWS - 1) / S::ROWS;
     const long long most = static_cast<long long>((p.keys_most + S::TILE - 1) / S::TILE) * p.batch * p.kv_heads * p.row_blocks;
-    const int ctas = static_cast<int>(std::min<long long>(CTAS, most));
-    p.part_lse = p.part_out + static_cast<size_t>(2 * CTAS) * S::ROWS * HEAD;
-    launch_chained(flash_decode_kernel<SOURCE, MT>, dim3(ctas), dim3(THREADS), S::BYTES, stream, p);
-    launch_chained(flash_decode_combine_kernel, dim3(p.kv_heads * p.group * p.tokens, p.batch), dim3(THREADS), 0, stream, p, S::TILE, S::ROWS, ctas);
+    if (most > 0x7fffffffLL) {
+        throw std::invalid_argument("flash attention over few rows: the shape exceeds the supported index range");
+    }
+    const int ctas = static_cast<int>(std::min<long long>(148LL * S::CTAS_PER_SM, most));
+    p.part_lse = p.part_out + static_cast<size_t>(2 * MOST_CTAS) * S::ROWS * HEAD;
+    p.notes = reinterpret_cast<PartNote*>(p.part_lse + static_cast<size_t>(2 * MOST_CTAS) * S::ROWS);
+    launch_chained(flash_decode_kernel<SOURCE, NB>, dim3(ctas), dim3(THREADS), S::BYTES, stream, p);
+    launch_chained(flash_decode_combine_kernel, dim3((p.kv_heads * rows + WARPS - 1) / WARPS, p.batch), dim3(THREADS), 0, stream, p, S::ROWS);
 }
 
 template <int SOURCE>
 void launch_rows(DecodeParams& p, cudaStream_t stream) {
-    if (p.group * p.tokens <= 16) {
-        launch_decode<SOURCE, 1>(p, stream);
-    } else {
-        launch_decode<SOURCE, 2>(p, stream);
+    switch (blocks_of_rows(static_cast<long long>(p.group) * p.tokens)) {
+        case 1:
+            return launch_decode<SOURCE, 1>(p, stream);
+        case 2:
+            return launch_decode<SOURCE, 2>(p, stream);
+        default:
+            return launch_decode<SOURCE, 4>(p, stream);
     }
 }
 
@@ -785,8 +812,10 @@ void launch_rows(DecodeParams& p, cudaStream_t stream) {
 
 namespace internal {
 
-std::size_t few_rows_workspace_bytes(long long rows) {
-    return static_cast<std::size_t>(2 * CTAS) * (rows <= 16 ? 16 : 32) * (HEAD + 1) * sizeof(float);
+std::size_t few_rows_workspace_bytes(int batch, int key_value_heads, long long rows) {
+    const std::size_t block = 8 * static_cast<std::size_t>(blocks_of_rows(rows));
+    const std::size_t items = static_cast<std::size_t>(batch) * key_value_heads * ((rows + block - 1) / block);
+    return 2 * MOST_CTAS * block * (HEAD + 1) * sizeof(float) + items * sizeof(PartNote);
 }
 
 void launch_few_rows_cross(__nv_bfloat16* output, float* logsumexp, const __nv_bfloat16* query, const __nv_bfloat16* key, const __nv_bfloat16* value,
@@ -824,11 +853,11 @@ int flash_decode_device_status(bool reset) {
 
 }  // namespace internal
 
-std::size_t flash_decode_workspace_bytes(int tokens, int query_heads, int key_value_heads) {
-    if (tokens <= 0 || query_heads <= 0 || key_value_heads <= 0) {
+std::size_t flash_decode_workspace_bytes(int batch_size, int tokens, int query_heads, int key_value_heads) {
+    if (batch_size <= 0 || tokens <= 0 || query_heads <= 0 || key_value_heads <= 0) {
         return 0;
     }
-    return internal::few_rows_workspace_bytes(static_cast<long long>(tokens) * (query_heads / key_value_heads));
+    return internal::few_rows_workspace_bytes(batch_size, key_value_heads, static_cast<long long>(tokens) * (query_heads / key_value_heads));
 }
 
 void flash_decode_cuda(__nv_bfloat16* output, float* logsumexp, const __nv_bfloat16* query, const void* key_cache, const void* value_cache,
@@ -849,7 +878,7 @@ void flash_decode_cuda(__nv_bfloat16* output, float* logsumexp, const __nv_bfloa
         throw std::invalid_argument("flash decode shape exceeds the supported index range");
     }
     internal::check_flash_pointers({output, query, key_cache, value_cache, workspace}, {logsumexp, key_scale, value_scale, block_table, cache_lengths});
-    if (workspace_bytes < flash_decode_workspace_bytes(tokens, query_heads, key_value_heads)) {
+    if (workspace_bytes < flash_decode_workspace_bytes(batch_size, tokens, query_heads, key_value_heads)) {
         throw std::invalid_argument("flash decode workspace is too small");
     }
     DecodeParams p{};

@@ -64,8 +64,8 @@ extern "C" int dscuda_flash_cache_append(void* key_cache, void* value_cache, flo
     });
 }
 
-extern "C" std::size_t dscuda_flash_decode_workspace_bytes(int tokens, int query_heads, int key_value_heads) {
-    return dscuda::flash_decode_workspace_bytes(tokens, query_heads, key_value_heads);
+extern "C" std::size_t dscuda_flash_decode_workspace_bytes(int batch, int tokens, int query_heads, int key_value_heads) {
+    return dscuda::flash_decode_workspace_bytes(batch, tokens, query_heads, key_value_heads);
 }
 
 extern "C" int dscuda_flash_decode(__nv_bfloat16* output, float* logsumexp, const __nv_bfloat16* query, const void* key_cache,

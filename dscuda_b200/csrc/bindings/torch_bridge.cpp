@@ -767,7 +767,7 @@ DSCUDA_FUNCTION(flash_decode) {
         expect_input(table, query, at::kInt, {b, table.size(1)}, "the block table");
         expect_input(lengths, query, at::kInt, {b}, "cache_lengths");
         const float scale = number(args[7]);
-        const size_t bytes = dscuda_flash_decode_workspace_bytes(static_cast<int>(t), static_cast<int>(hq), cache.heads);
+        const size_t bytes = dscuda_flash_decode_workspace_bytes(static_cast<int>(b), static_cast<int>(t), static_cast<int>(hq), cache.heads);
         const Tensor* workspace_given = optional_workspace(args[8], query, bytes);
         const Tensor *output_given = optional_output(args[9], query, at::kBFloat16, query.numel(), "the output"),
                      *lse_given = optional_output(args[10], query, at::kFloat, b * hq * t, "the LSE");

@@ -42,9 +42,9 @@ def cache_append(key_cache, value_cache, key_scale, value_scale, key, value, blo
     extension().flash_cache_append(key_cache, value_cache, key_scale, value_scale, key, value, block_table, start_positions, token_counts)
 
 
-def decode_workspace(tokens, query_heads, key_value_heads, device="cuda"):
+def decode_workspace(batch, tokens, query_heads, key_value_heads, device="cuda"):
     """Workspace of `decode` for calls of these sizes.  Calls that may run at the same time need one each."""
-    return torch.empty(library("flash_attention").dscuda_flash_decode_workspace_bytes(tokens, query_heads, key_value_heads), device=device,
+    return torch.empty(library("flash_attention").dscuda_flash_decode_workspace_bytes(batch, tokens, query_heads, key_value_heads), device=device,
                        dtype=torch.uint8)
 
 

@@ -49,7 +49,7 @@ FLASH_SYMBOLS = {
     "dscuda_flash_forward": ([P] * 5 + [I] * 5 + [F, P], I),
     "dscuda_flash_rope": ([P] * 5 + [L] + [I] * 3 + [L] * 4 + [I, P, I, I, F, P], I),
     "dscuda_flash_cache_append": ([P] * 9 + [I] * 4 + [L] * 2 + [I] * 4 + [P], I),
-    "dscuda_flash_decode_workspace_bytes": ([I] * 3, Z),
+    "dscuda_flash_decode_workspace_bytes": ([I] * 4, Z),
     "dscuda_flash_decode": ([P] * 10 + [Z] + [I] * 9 + [F, P], I),
     "dscuda_flash_cross_forward_workspace_bytes": ([I] * 5, Z),
     "dscuda_flash_cross_forward": ([P] * 7 + [Z] + [I] * 6 + [F, P], I),

@@ -191,7 +191,7 @@ int dscuda_flash_cache_append(
     int page_size, int pages, int cache_blocks, int type, void* stream);
 
 /* No counterpart in the reference (flash_decode_workspace_bytes, flash_decode_cuda). */
-size_t dscuda_flash_decode_workspace_bytes(int tokens, int query_heads, int key_value_heads);
+size_t dscuda_flash_decode_workspace_bytes(int batch, int tokens, int query_heads, int key_value_heads);
 int dscuda_flash_decode(
     void* output, float* lse, const void* query, const void* key_cache, const void* value_cache,
     const float* key_scale, const float* value_scale, const int* block_table, const int* lengths,

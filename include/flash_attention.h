@@ -100,8 +100,8 @@ void flash_cache_append_cuda(
     FlashCacheType type,
     cudaStream_t stream = nullptr);
 
-// Bytes of the decode's workspace (depends on the rows to a key head, tokens * Hq / Hkv, alone).
-std::size_t flash_decode_workspace_bytes(int tokens, int query_heads, int key_value_heads);
+// Bytes of the decode's workspace.
+std::size_t flash_decode_workspace_bytes(int batch_size, int tokens, int query_heads, int key_value_heads);
 
 // Attention of the newest T tokens (at most FLASH_DECODE_MAX_TOKENS) over that cache.  query, output [B,T,Hq,128], logsumexp [B,Hq,T].
 // cache_lengths [B] counts the new tokens too: token t sees the first cache_lengths[b] - T + 1 + t positions.  A row that sees

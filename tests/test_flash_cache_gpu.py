@@ -204,7 +204,7 @@ def test_the_same_bits_again_and_given_memory(gpu):
     table = tables(3, 23, 70, 42).to(gpu)
     query, lengths = normal(43, 3, 2, 16, 128).to(gpu), torch.tensor([1400, 3, 700], dtype=torch.int32, device=gpu)
     first = flash.decode(query, *cache, table, lengths, SCALE)
-    workspace = flash.decode_workspace(2, 16, 4, gpu).fill_(0xff)
+    workspace = flash.decode_workspace(3, 2, 16, 4, gpu).fill_(0xff)
     out, lse = torch.empty_like(query), torch.empty(3, 16, 2, device=gpu)
     flash.decode(query, *cache, table, lengths, SCALE, workspace, out, lse)
     assert torch.equal(first[0], out) and torch.equal(first[1], lse)
