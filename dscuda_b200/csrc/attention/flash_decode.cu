@@ -14,7 +14,7 @@
 //
 // Operands.  Codes become f16 (exact for both types: int8 through 1024 + u - 1152, e4m3 by conversion) and so does Q, each row
 // multiplied by a power of two that brings its largest element to 2^13..2^14; P is rounded to f16 (half a step is 2^-11 of it), relative to the
-// largest value scale met so far and times 2^14, so that small weights of long rows keep their bits.  bf16 states are multiplied as they
+// largest value scale met so far and times 2^7, so that small weights of long rows keep their bits (the smallest step is 2^-31 of the largest weight).  bf16 states are multiplied as they
 // are, P rounded to bf16.  Sums, maxima and the softmax are fp32.
 //
 // Products.  S^T = K Q^T and O^T = V^T P^T: the keys, and then the head columns, are the 16 rows of an instruction, the query rows its 8
@@ -54,7 +54,9 @@ constexpr int MOST_CTAS = 3 * 148;
 constexpr int MERGE_PITCH = HEAD + 4;       // floats between rows of the merge buffer
 constexpr float LOG2E = 1.4426950408889634F;
 constexpr float LN2 = 0.6931471805599453F;
-constexpr float WEIGHT_UNIT = 16384.0F;     // f16 weights are stored times this
+constexpr float WEIGHT_UNIT = 128.0F;       // f16 weights are stored times this
+constexpr float RESCALE_THRESHOLD = 8.0F;   // log2 units by which a score may pass the reference before the sums are rescaled; f16 holds 2^8 * 128
+constexpr unsigned ITEM_TILES = 1;          // what an item costs beside its tiles (Q, pipeline fill, merge), in tiles
 
 enum Source { INT8 = 0, E4M3 = 1, BF16 = 2 };
 
@@ -174,6 +176,11 @@ __device__ __forceinline__ int length_of(const DecodeParams& p, int b) {
     return min(max(length, 0), p.keys_most);
 }
 
+// What an item of `length` keys counts when the ranges are cut: its tiles and ITEM_TILES in front of them.
+__device__ __forceinline__ unsigned item_cost(int length, int tile) {
+    return length > 0 ? (length + tile - 1) / tile + ITEM_TILES : 0;
+}
+
 // The address of a query or output row: row = token * group + head of the group.
 __device__ __forceinline__ size_t row_offset(const DecodeParams& p, int b, int kv_head, int row) {
     const int token = row / p.group;
@@ -227,10 +234,10 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
     const unsigned items = p.kv_heads * p.row_blocks;
     unsigned total = 0;
     for (int base = 0; base < p.batch; base += 32) {
-        unsigned tiles = base + lane < p.batch ? (length_of(p, base + lane) + S::TILE - 1) / S::TILE * items : 0;
-        total += __reduce_add_sync(0xffffffffU, tiles);
+        const unsigned cost = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
+        total += __reduce_add_sync(0xffffffffU, cost);
     }
-    const unsigned ctas = min(total, gridDim.x);        // with a tile each
+    const unsigned ctas = min(total, gridDim.x);
     if (blockIdx.x >= ctas) {
         return;
     }
@@ -240,7 +247,7 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
     unsigned entry_first = 0;
     int entry = 0;
     for (int base = 0;; base += 32) {
-        const unsigned own = base + lane < p.batch ? (length_of(p, base + lane) + S::TILE - 1) / S::TILE * items : 0;
+        const unsigned own = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
         unsigned inclusive = own;
 #pragma unroll
         for (int offset = 1; offset < 32; offset <<= 1) {
@@ -260,16 +267,21 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
     bool first_segment = true;
     while (position < end) {
         const int length = length_of(p, entry);
-        const unsigned entry_tiles = (length + S::TILE - 1) / S::TILE;
-        if (position >= entry_first + entry_tiles * items) {
-            entry_first += entry_tiles * items;
+        const unsigned cost = item_cost(length, S::TILE);
+        if (position >= entry_first + cost * items) {
+            entry_first += cost * items;
             ++entry;
             continue;
         }
-        const unsigned item = (position - entry_first) / entry_tiles;
-        const unsigned item_first = entry_first + item * entry_tiles;
-        const int tile_begin = static_cast<int>(position - item_first);
-        const int tile_end = static_cast<int>(min(entry_tiles, end - item_first));
+        const unsigned item = (position - entry_first) / cost;
+        const unsigned first_tile = entry_first + item * cost + ITEM_TILES;         // position of the item's first tile
+        const int entry_tiles = static_cast<int>(cost - ITEM_TILES);
+        const int tile_begin = static_cast<int>(max(position, first_tile) - first_tile);
+        const int tile_end = min(entry_tiles, static_cast<int>(end) - static_cast<int>(first_tile));
+        position = first_tile + max(tile_end, 0);
+        if (tile_end <= tile_begin) {
+            continue;                   // the range ends in front of the item's tiles
+        }
         const int kv_head = static_cast<int>(item) / p.row_blocks;
         const int row_base = (static_cast<int>(item) - kv_head * p.row_blocks) * S::ROWS;
         const int rows = p.group * p.tokens;
@@ -313,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                         const size_t offset = static_cast<size_t>(at) * 128 + lane * 16;        // rows of a group lie one after the other
                         const uint8_t *k = p.keys + offset, *v = p.values + offset;
                         const int left = length - key0 - 16 * u;
-                        if (left >= 16) {
+                        if (__all_sync(0xffffffffU, left >= 16)) {
 #pragma unroll
                             for (int i = 0; i < 4; ++i) {
                                 const uint32_t to = copy_to[i % 2] + slot + (16 * u + 8 * (i / 2)) * 128;
@@ -394,7 +406,8 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
             for (int side = 0; side < 2; ++side) {
                 const int column = row_base + nb * 8 + 2 * c + side;
                 factor[nb][side] = __shfl_sync(0xffffffffU, down, 8 * c + 4 * side);
-                limit[nb][side] = column < rows ? (p.causal ? length - p.tokens + 1 + column / p.group : length) : 0;
+                // (rows that do not exist have Q = 0 and are not written)
+                limit[nb][side] = p.causal && column < rows ? length - p.tokens + 1 + column / p.group : length;
                 least = min(least, limit[nb][side]);
             }
 #pragma unroll
@@ -510,15 +523,16 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                     value_scale[u] = meta.value[u] * inverse;
                 }
             }
+            // The reference m of a row lags its maximum by up to the threshold: the lanes of a row compare notes, and the sums are rescaled,
+            // only when one of them passes it.
             const bool masked = key0 + KEYS > least;
-            uint2 weights[KU][NB];
+            float top[NB][2];
             bool moved = shrink != 1.0F;
-            float alpha[NB][2];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
                 for (int side = 0; side < 2; ++side) {
-                    float top = -INFINITY;
+                    top[nb][side] = -INFINITY;
 #pragma unroll
                     for (int u = 0; u < KU; ++u) {
                         const float f = factor[nb][side] * key_scale[u];
@@ -528,16 +542,42 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                             score[u][nb][side] = key0 + 16 * u + g < limit[nb][side] ? score[u][nb][side] : -INFINITY;
                             score[u][nb][2 + side] = key0 + 16 * u + 8 + g < limit[nb][side] ? score[u][nb][2 + side] : -INFINITY;
                         }
-                        top = sm100::max3(top, score[u][nb][side], score[u][nb][2 + side]);
+                        top[nb][side] = sm100::max3(top[nb][side], score[u][nb][side], score[u][nb][2 + side]);
+                    }
+                    moved |= top[nb][side] > m[nb][side] + RESCALE_THRESHOLD;
+                }
+            }
+            if (__any_sync(0xffffffffU, moved)) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    float alpha[2];
+#pragma unroll
+                    for (int side = 0; side < 2; ++side) {
+#pragma unroll
+                        for (int offset = 4; offset < 32; offset <<= 1) {
+                            top[nb][side] = fmaxf(top[nb][side], __shfl_xor_sync(0xffffffffU, top[nb][side], offset));
+                        }
+                        const float now = fmaxf(m[nb][side], top[nb][side]);
+                        alpha[side] = now == -INFINITY ? 1.0F : exp2_approx(m[nb][side] - now);         // no key so far: the sums are zero
+                        m[nb][side] = now;
+                        l[nb][side] *= alpha[side];
+                        alpha[side] *= shrink;
                     }
 #pragma unroll
-                    for (int offset = 4; offset < 32; offset <<= 1) {
-                        top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, offset));
+                    for (int j = 0; j < 8; ++j) {
+                        o[nb][j][0] *= alpha[0];
+                        o[nb][j][1] *= alpha[1];
+                        o[nb][j][2] *= alpha[0];
+                        o[nb][j][3] *= alpha[1];
                     }
-                    const float now = fmaxf(m[nb][side], top);
-                    const float reference = now == -INFINITY ? 0.0F : now;          // no key so far: all weights are exp2(-inf) = 0
-                    alpha[nb][side] = exp2_approx(m[nb][side] - reference);
-                    m[nb][side] = now;
+                }
+            }
+            uint2 weights[KU][NB];
+#pragma unroll
+            for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                for (int side = 0; side < 2; ++side) {
+                    const float reference = m[nb][side] == -INFINITY ? 0.0F : m[nb][side];         // all weights are exp2(-inf) = 0
                     float sum = 0.0F;
 #pragma unroll
                     for (int u = 0; u < KU; ++u) {
@@ -548,27 +588,13 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                             score[u][nb][2 * h + side] = SOURCE == BF16 ? weight : weight * value_scale[u];
                         }
                     }
-                    l[nb][side] = l[nb][side] * alpha[nb][side] + sum;
-                    alpha[nb][side] *= shrink;
-                    moved |= alpha[nb][side] != 1.0F;
+                    l[nb][side] += sum;
                 }
 #pragma unroll
                 for (int u = 0; u < KU; ++u) {
                     const float(&x)[4] = score[u][nb];
                     weights[u][nb].x = turn8x8(SOURCE == BF16 ? sm100::pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]));
                     weights[u][nb].y = turn8x8(SOURCE == BF16 ? sm100::pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]));
-                }
-            }
-            if (__any_sync(0xffffffffU, moved)) {
-#pragma unroll
-                for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) {
-                        o[nb][j][0] *= alpha[nb][0];
-                        o[nb][j][1] *= alpha[nb][1];
-                        o[nb][j][2] *= alpha[nb][0];
-                        o[nb][j][3] *= alpha[nb][1];
-                    }
                 }
             }
 
@@ -643,10 +669,10 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
             merge_unit[warp] = SOURCE == BF16 ? 1.0F : unit / WEIGHT_UNIT;
         }
         __syncthreads();
-        const bool whole = tile_begin == 0 && tile_end == static_cast<int>(entry_tiles);
+        const bool whole = tile_begin == 0 && tile_end == entry_tiles;
         const unsigned slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
         if (tile_begin == 0 && threadIdx.x == 0) {
-            const int holders = static_cast<int>(ranges.holder(item_first + entry_tiles - 1) - blockIdx.x) + 1;
+            const int holders = static_cast<int>(ranges.holder(first_tile + entry_tiles - 1) - blockIdx.x) + 1;
             p.notes[static_cast<size_t>(entry) * items + item] = {static_cast<int>(blockIdx.x), 2 * holders + (first_segment ? 0 : 1)};
         }
         constexpr int PER_ROW = THREADS / 8;            // threads to a row
@@ -699,7 +725,6 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                 }
             }
         }
-        position = item_first + tile_end;
         first_segment = false;
     }
 }
@@ -785,7 +810,7 @@ void launch_decode(DecodeParams& p, cudaStream_t stream) {
     }
     const int rows = p.group * p.tokens;
     p.row_blocks = (rows + S::ROWS - 1) / S::ROWS;
-    const long long most = static_cast<long long>((p.keys_most + S::TILE - 1) / S::TILE) * p.batch * p.kv_heads * p.row_blocks;
+    const long long most = static_cast<long long>((p.keys_most + S::TILE - 1) / S::TILE + ITEM_TILES) * p.batch * p.kv_heads * p.row_blocks;
     if (most > 0x7fffffffLL) {
         throw std::invalid_argument("flash attention over few rows: the shape exceeds the supported index range");
     }

@@ -95,8 +95,8 @@ def attention(query, keys, values, scale, limits, weight_step):
     out = torch.einsum("htn,nhd->thd", p, v)
     weighed = torch.einsum("htn,nhd->thd", p, v.abs())
     relative = (weight_step + EXP + 2 * ds).t()[..., None]
-    # weights far below the largest one lose bits in f16: at most 2^-39 of it each
-    out_slack = BF16 * out.abs() + (1 + BF16) * relative * weighed + k.shape[0] * 2.0 ** -39 * v.abs().amax()
+    # weights far below the largest one lose bits in f16: at most 2^-32 of it each
+    out_slack = BF16 * out.abs() + (1 + BF16) * relative * weighed + k.shape[0] * 2.0 ** -32 * v.abs().amax()
     lse_slack = ds + EXP + 2.0 ** -22 * torch.where(torch.isfinite(lse), lse, 0.0).abs()
     return out, lse, out_slack, lse_slack
 
