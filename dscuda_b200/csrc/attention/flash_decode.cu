@@ -35,8 +35,6 @@
 #include "../common/launch.h"
 
 #include <cuda_fp16.h>
-#include <cuda_fp8.h>
-
 #include <algorithm>
 #include <cstdint>
 #include <stdexcept>
@@ -160,10 +158,14 @@ __device__ __forceinline__ void widen(uint32_t word, uint32_t& lo, uint32_t& hi)
         lo = *reinterpret_cast<const uint32_t*>(&dl);
         hi = *reinterpret_cast<const uint32_t*>(&dh);
     } else {
-        const __half2_raw dl = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(word & 0xffffU), __NV_E4M3);
-        const __half2_raw dh = __nv_cvt_fp8x2_to_halfraw2(static_cast<__nv_fp8x2_storage_t>(word >> 16), __NV_E4M3);
-        lo = static_cast<uint32_t>(dl.x) | (static_cast<uint32_t>(dl.y) << 16);
-        hi = static_cast<uint32_t>(dh.x) | (static_cast<uint32_t>(dh.y) << 16);
+        asm("{\n\t"
+            ".reg .b16 l, h;\n\t"
+            "mov.b32 {l, h}, %2;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %0, l;\n\t"
+            "cvt.rn.f16x2.e4m3x2 %1, h;\n\t"
+            "}\n"
+            : "=r"(lo), "=r"(hi)
+            : "r"(word));
     }
 }
 
@@ -432,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
         };
 
         float o[NB][8][4];              // O^T: m-tile j holds head columns 2 j and 2 j + 1 of the lane's unit; query rows 2 c and 2 c + 1
-        float m[NB][2], l[NB][2];
+        float2 m[NB], l[NB];            // reference and sum of rows 2 c and 2 c + 1 (the sum over this lane's keys)
         float unit = 0.0F;              // the largest value scale so far: weights are relative to it
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
@@ -443,8 +445,8 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                     o[nb][j][e] = 0.0F;
                 }
             }
-            m[nb][0] = m[nb][1] = -INFINITY;
-            l[nb][0] = l[nb][1] = 0.0F;
+            m[nb] = make_float2(-INFINITY, -INFINITY);
+            l[nb] = make_float2(0.0F, 0.0F);
         }
         for (int s = 0; s < steps; ++s) {
             __syncwarp();               // every lane has read the slot that is filled next
@@ -525,76 +527,86 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
             }
             // The reference m of a row lags its maximum by up to the threshold: the lanes of a row compare notes, and the sums are rescaled,
             // only when one of them passes it.
-            const bool masked = key0 + KEYS > least;
-            float top[NB][2];
+            // x = score * f - reference for the pair of query rows at once.  The reference m of a row lags its maximum by up to the threshold: the
+            // lanes of a row compare notes, and the sums are rescaled, only when one of them passes it.
+            float2 f[KU][NB];
+#pragma unroll
+            for (int u = 0; u < KU; ++u) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+                    f[u][nb] = make_float2(factor[nb][0] * key_scale[u], factor[nb][1] * key_scale[u]);
+                }
+            }
+            if (__any_sync(0xffffffffU, key0 + KEYS > least)) {
+#pragma unroll
+                for (int nb = 0; nb < NB; ++nb) {
+#pragma unroll
+                    for (int u = 0; u < KU; ++u) {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float x = score[u][nb][e] * (e % 2 == 0 ? f[u][nb].x : f[u][nb].y);
+                            score[u][nb][e] = key0 + 16 * u + 8 * (e / 2) + g < limit[nb][e % 2] ? x : -INFINITY;
+                        }
+                        f[u][nb] = make_float2(1.0F, 1.0F);         // (a scale of zero must not meet the infinity)
+                    }
+                }
+            }
+            float2 top[NB];
             bool moved = shrink != 1.0F;
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
+                top[nb] = make_float2(-INFINITY, -INFINITY);
 #pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                    top[nb][side] = -INFINITY;
-#pragma unroll
-                    for (int u = 0; u < KU; ++u) {
-                        const float f = factor[nb][side] * key_scale[u];
-                        score[u][nb][side] *= f;
-                        score[u][nb][2 + side] *= f;
-                        if (masked) {
-                            score[u][nb][side] = key0 + 16 * u + g < limit[nb][side] ? score[u][nb][side] : -INFINITY;
-                            score[u][nb][2 + side] = key0 + 16 * u + 8 + g < limit[nb][side] ? score[u][nb][2 + side] : -INFINITY;
-                        }
-                        top[nb][side] = sm100::max3(top[nb][side], score[u][nb][side], score[u][nb][2 + side]);
-                    }
-                    moved |= top[nb][side] > m[nb][side] + RESCALE_THRESHOLD;
+                for (int u = 0; u < KU; ++u) {
+                    top[nb].x = fmaxf(top[nb].x, fmaxf(score[u][nb][0], score[u][nb][2]) * f[u][nb].x);
+                    top[nb].y = fmaxf(top[nb].y, fmaxf(score[u][nb][1], score[u][nb][3]) * f[u][nb].y);
                 }
+                moved |= top[nb].x > m[nb].x + RESCALE_THRESHOLD || top[nb].y > m[nb].y + RESCALE_THRESHOLD;
             }
             if (__any_sync(0xffffffffU, moved)) {
 #pragma unroll
                 for (int nb = 0; nb < NB; ++nb) {
-                    float alpha[2];
 #pragma unroll
-                    for (int side = 0; side < 2; ++side) {
-#pragma unroll
-                        for (int offset = 4; offset < 32; offset <<= 1) {
-                            top[nb][side] = fmaxf(top[nb][side], __shfl_xor_sync(0xffffffffU, top[nb][side], offset));
-                        }
-                        const float now = fmaxf(m[nb][side], top[nb][side]);
-                        alpha[side] = now == -INFINITY ? 1.0F : exp2_approx(m[nb][side] - now);         // no key so far: the sums are zero
-                        m[nb][side] = now;
-                        l[nb][side] *= alpha[side];
-                        alpha[side] *= shrink;
+                    for (int offset = 4; offset < 32; offset <<= 1) {
+                        top[nb].x = fmaxf(top[nb].x, __shfl_xor_sync(0xffffffffU, top[nb].x, offset));
+                        top[nb].y = fmaxf(top[nb].y, __shfl_xor_sync(0xffffffffU, top[nb].y, offset));
                     }
+                    const float2 now = make_float2(fmaxf(m[nb].x, top[nb].x), fmaxf(m[nb].y, top[nb].y));
+                    // no key so far: the sums are zero
+                    float2 alpha = make_float2(now.x == -INFINITY ? 1.0F : exp2_approx(m[nb].x - now.x), now.y == -INFINITY ? 1.0F : exp2_approx(m[nb].y - now.y));
+                    m[nb] = now;
+                    l[nb] = make_float2(l[nb].x * alpha.x, l[nb].y * alpha.y);
+                    alpha = make_float2(alpha.x * shrink, alpha.y * shrink);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
-                        o[nb][j][0] *= alpha[0];
-                        o[nb][j][1] *= alpha[1];
-                        o[nb][j][2] *= alpha[0];
-                        o[nb][j][3] *= alpha[1];
+                        o[nb][j][0] *= alpha.x;
+                        o[nb][j][1] *= alpha.y;
+                        o[nb][j][2] *= alpha.x;
+                        o[nb][j][3] *= alpha.y;
                     }
                 }
             }
             uint2 weights[KU][NB];
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) {
-#pragma unroll
-                for (int side = 0; side < 2; ++side) {
-                    const float reference = m[nb][side] == -INFINITY ? 0.0F : m[nb][side];         // all weights are exp2(-inf) = 0
-                    float sum = 0.0F;
-#pragma unroll
-                    for (int u = 0; u < KU; ++u) {
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            const float weight = exp2_approx(score[u][nb][2 * h + side] - reference);
-                            sum += weight;
-                            score[u][nb][2 * h + side] = SOURCE == BF16 ? weight : weight * value_scale[u];
-                        }
-                    }
-                    l[nb][side] += sum;
-                }
+                // a row without any key so far: all its weights are exp2(-inf) = 0
+                const float2 minus = make_float2(m[nb].x == -INFINITY ? 0.0F : -m[nb].x, m[nb].y == -INFINITY ? 0.0F : -m[nb].y);
 #pragma unroll
                 for (int u = 0; u < KU; ++u) {
-                    const float(&x)[4] = score[u][nb];
-                    weights[u][nb].x = turn8x8(SOURCE == BF16 ? sm100::pack_bf16x2(x[0], x[1]) : pack_f16x2(x[0], x[1]));
-                    weights[u][nb].y = turn8x8(SOURCE == BF16 ? sm100::pack_bf16x2(x[2], x[3]) : pack_f16x2(x[2], x[3]));
+                    uint32_t packed[2];
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        const float2 x = sm100::fma2(make_float2(score[u][nb][2 * h], score[u][nb][2 * h + 1]), f[u][nb], minus);
+                        const float2 weight = make_float2(exp2_approx(x.x), exp2_approx(x.y));
+                        l[nb] = sm100::add2(l[nb], weight);
+                        if constexpr (SOURCE == BF16) {
+                            packed[h] = sm100::pack_bf16x2(weight.x, weight.y);
+                        } else {
+                            const float2 scaled = sm100::mul2(weight, make_float2(value_scale[u], value_scale[u]));
+                            packed[h] = pack_f16x2(scaled.x, scaled.y);
+                        }
+                    }
+                    weights[u][nb] = make_uint2(turn8x8(packed[0]), turn8x8(packed[1]));
                 }
             }
 
@@ -647,14 +659,14 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
         for (int nb = 0; nb < NB; ++nb) {
 #pragma unroll
             for (int side = 0; side < 2; ++side) {
-                float sum = l[nb][side];
+                float sum = side == 0 ? l[nb].x : l[nb].y;
 #pragma unroll
                 for (int offset = 4; offset < 32; offset <<= 1) {
                     sum += __shfl_xor_sync(0xffffffffU, sum, offset);
                 }
                 const int row = nb * 8 + 2 * c + side;
                 if (g == 0) {
-                    merge_m[warp][row] = m[nb][side];
+                    merge_m[warp][row] = side == 0 ? m[nb].x : m[nb].y;
                     merge_l[warp][row] = sum;
                 }
                 float* dst = merge + (warp * S::ROWS + row) * MERGE_PITCH;

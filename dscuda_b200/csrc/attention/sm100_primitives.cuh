@@ -564,6 +564,21 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     return result;
 }
 
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    unsigned long long ra;
+    asm("{\n\t"
+        ".reg .b64 x, y;\n\t"
+        "mov.b64 x, {%1, %2};\n\t"
+        "mov.b64 y, {%3, %4};\n\t"
+        "mul.rn.f32x2 %0, x, y;\n\t"
+        "}\n"
+        : "=l"(ra)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    float2 result;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(result.x), "=f"(result.y) : "l"(ra));
+    return result;
+}
+
 __device__ __forceinline__ float max3(float a, float b, float c) {
     float result;
     asm("max.f32 %0, %1, %2, %3;" : "=f"(result) : "f"(a), "f"(b), "f"(c));

@@ -62,7 +62,7 @@ void flash_rope_cuda(
     cudaStream_t stream = nullptr);
 
 // The paged cache in 8 bits: keys and values each as codes [cache_blocks, Hkv, page_size, 128] with one FP32 scale for each page and
-// head, [cache_blocks, Hkv]; value = code * scale.  page_size is a multiple of 16.
+// head, [cache_blocks, Hkv]; value = code * scale, scales are not negative.  page_size is a multiple of 16.
 enum class FlashCacheType : int {
     INT8 = 0,           // codes -127..127
     E4M3 = 1,           // codes up to +-448
