@@ -31,6 +31,7 @@ constexpr int THREADS = 128;
 constexpr int ROWS_PER_PASS = THREADS / 16;         // 16 lanes x 16 bytes of bf16 to a row
 constexpr int HELD = 8;                             // passes whose rows stay in registers; larger pages read the rest again (from L2)
 constexpr float SMALLEST = 7.888609052210118e-31F;  // 2^-100
+constexpr uint32_t INFINITE = 0x7f80;               // bf16 magnitudes from here on are infinities and NaN
 
 __device__ int flash_cache_status = 0;
 
@@ -45,14 +46,36 @@ struct AppendParams {
     int tokens, kv_heads, page, pages, blocks;
 };
 
+__device__ __forceinline__ float low_bf16(uint32_t pair) {
+    return __uint_as_float(pair << 16);
+}
+
+__device__ __forceinline__ float high_bf16(uint32_t pair) {
+    return __uint_as_float(pair & 0xffff0000U);
+}
+
+// Four codes of finite values that lie in the type's range (up to the rounding of the product).
 template <bool INT8>
-__device__ __forceinline__ uint32_t encode(float x) {
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
     if constexpr (INT8) {
-        // fminf / fmaxf drop a NaN; __float2int_rn rounds half to even
-        return static_cast<uint32_t>(static_cast<uint8_t>(static_cast<int8_t>(__float2int_rn(fminf(fmaxf(x, -127.0F), 127.0F)))));
+        // 1.5 * 2^23 + x rounds x half to even into the lowest bits
+        constexpr float ROUND = 12582912.0F;
+        const uint32_t low = __byte_perm(__float_as_uint(__fadd_rn(a, ROUND)), __float_as_uint(__fadd_rn(b, ROUND)), 0x0040);
+        const uint32_t high = __byte_perm(__float_as_uint(__fadd_rn(c, ROUND)), __float_as_uint(__fadd_rn(d, ROUND)), 0x0040);
+        return __byte_perm(low, high, 0x5410);
     } else {
-        return __nv_cvt_float_to_fp8(x, __NV_SATFINITE, __NV_E4M3);
+        const uint32_t low = __nv_cvt_float2_to_fp8x2(make_float2(a, b), __NV_SATFINITE, __NV_E4M3);
+        const uint32_t high = __nv_cvt_float2_to_fp8x2(make_float2(c, d), __NV_SATFINITE, __NV_E4M3);
+        return low | (high << 16);
     }
+}
+
+// One code of any value: NaN is 0, infinities the largest codes.
+template <bool INT8>
+__device__ __forceinline__ uint32_t encode_any(float x) {
+    constexpr float LARGEST = INT8 ? 127.0F : 448.0F;
+    const float inside = isnan(x) ? 0.0F : fminf(fmaxf(x, -LARGEST), LARGEST);
+    return encode4<INT8>(inside, 0.0F, 0.0F, 0.0F) & 0xffU;
 }
 
 template <bool INT8>
@@ -64,18 +87,14 @@ __device__ __forceinline__ float decode(uint32_t code) {
     }
 }
 
-__device__ __forceinline__ float finite_magnitude(float x) {
-    return isfinite(x) ? fabsf(x) : 0.0F;
-}
-
 template <bool INT8>
 __global__ void __launch_bounds__(THREADS) flash_cache_append_kernel(const __grid_constant__ AppendParams p) {
     constexpr float LARGEST = INT8 ? 127.0F : 448.0F;
-    __shared__ float warp_max[THREADS / 32];
+    __shared__ uint32_t warp_max[2][THREADS / 32];
     const int b = blockIdx.z;
     const int side = blockIdx.y % 2;                // keys, values
     const int head = blockIdx.y / 2;
-    const int lane = threadIdx.x % 32;
+    const int warp = threadIdx.x / 32;
     sm100::grid_dependency_wait();
     const long long start = p.starts != nullptr ? p.starts[b] : 0;
     const long long count = p.counts != nullptr ? min(max(p.counts[b], 0), p.tokens) : p.tokens;
@@ -87,6 +106,18 @@ __global__ void __launch_bounds__(THREADS) flash_cache_append_kernel(const __gri
     if (begin >= end) {
         return;
     }
+    const int slot = static_cast<int>(begin - logical * p.page);        // of the first new row; the rows in front of it are older
+    const int rows = static_cast<int>(end - begin);
+    const __nv_bfloat16* source = p.rows[side] + (static_cast<long long>(b) * p.tokens + (begin - start)) * p.stride[side] + head * HEAD;
+    const int part = threadIdx.x % 16;
+    const int mine = threadIdx.x / 16;
+    auto load = [&](int row) { return *reinterpret_cast<const uint4*>(source + row * p.stride[side] + part * 8); };
+    uint4 held[HELD];
+#pragma unroll
+    for (int k = 0; k < HELD; ++k) {
+        const int row = k * ROWS_PER_PASS + mine;
+        held[k] = row < rows ? load(row) : make_uint4(0, 0, 0, 0);
+    }
     int physical = -1;
     if (logical < p.pages) {
         physical = p.table[static_cast<long long>(b) * p.pages + logical];
@@ -97,29 +128,31 @@ __global__ void __launch_bounds__(THREADS) flash_cache_append_kernel(const __gri
         }
         return;
     }
-    const int slot = static_cast<int>(begin - logical * p.page);        // of the first new row; the rows in front of it are older
-    const int rows = static_cast<int>(end - begin);
     const size_t head_page = static_cast<size_t>(physical) * p.kv_heads + head;
     uint8_t* page = p.cache[side] + head_page * p.page * HEAD;
-    const __nv_bfloat16* source = p.rows[side] + (static_cast<long long>(b) * p.tokens + (begin - start)) * p.stride[side] + head * HEAD;
-    const int part = threadIdx.x % 16;
-    const int mine = threadIdx.x / 16;
-    auto load = [&](int row) { return *reinterpret_cast<const uint4*>(source + row * p.stride[side] + part * 8); };
+    const float old = slot > 0 ? p.scale[side][head_page] : 0.0F;
 
-    uint4 held[HELD];
-    float largest = 0.0F;
-    auto measure = [&](const uint4& v) {
-        const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            largest = fmaxf(largest, fmaxf(finite_magnitude(__uint_as_float(words[e] << 16)), finite_magnitude(__uint_as_float(words[e] & 0xffff0000U))));
+    // the largest magnitude as bf16 bits, two at a time: their order is that of the integers, infinities and NaN on top
+    auto block_max = [&](uint32_t pairs, int round) {
+        const uint32_t top = __reduce_max_sync(0xffffffffU, max(pairs & 0xffffU, pairs >> 16));
+        if (threadIdx.x % 32 == 0) {
+            warp_max[round][warp] = top;
         }
-    };
+        __syncthreads();
+        uint32_t largest = 0;
 #pragma unroll
-    for (int k = 0; k < HELD; ++k) {
-        const int row = k * ROWS_PER_PASS + mine;
-        held[k] = row < rows ? load(row) : make_uint4(0, 0, 0, 0);
-    }
+        for (int w = 0; w < THREADS / 32; ++w) {
+            largest = max(largest, warp_max[round][w]);
+        }
+        return largest;
+    };
+    uint32_t pairs = 0;
+    auto measure = [&](const uint4& v) {
+        pairs = __vmaxu2(pairs, v.x & 0x7fff7fffU);
+        pairs = __vmaxu2(pairs, v.y & 0x7fff7fffU);
+        pairs = __vmaxu2(pairs, v.z & 0x7fff7fffU);
+        pairs = __vmaxu2(pairs, v.w & 0x7fff7fffU);
+    };
 #pragma unroll
     for (int k = 0; k < HELD; ++k) {
         measure(held[k]);
@@ -127,33 +160,41 @@ __global__ void __launch_bounds__(THREADS) flash_cache_append_kernel(const __gri
     for (int row = HELD * ROWS_PER_PASS + mine; row < rows; row += ROWS_PER_PASS) {
         measure(load(row));
     }
-    const float old = slot > 0 ? p.scale[side][head_page] : 0.0F;
-#pragma unroll
-    for (int offset = 16; offset > 0; offset >>= 1) {
-        largest = fmaxf(largest, __shfl_xor_sync(0xffffffffU, largest, offset));
+    uint32_t largest_bits = block_max(pairs, 0);
+    const bool finite = largest_bits < INFINITE;
+    if (!finite) {
+        // again without the values that are not finite
+        pairs = 0;
+        for (int row = mine; row < rows; row += ROWS_PER_PASS) {
+            const uint4 v = load(row);
+            const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t low = words[e] & 0x7fffU, high = (words[e] >> 16) & 0x7fffU;
+                pairs = __vmaxu2(pairs, (low < INFINITE ? low : 0) | (high < INFINITE ? high << 16 : 0));
+            }
+        }
+        largest_bits = block_max(pairs, 1);
     }
-    if (lane == 0) {
-        warp_max[threadIdx.x / 32] = largest;
-    }
-    __syncthreads();
-    for (int w = 0; w < THREADS / 32; ++w) {
-        largest = fmaxf(largest, warp_max[w]);
-    }
+    const float largest = __uint_as_float(largest_bits << 16);
     const float need = largest < SMALLEST ? 0.0F : __fmul_rn(largest, 1.0F / LARGEST);
     const float scale = fmaxf(old, need);
     const float inverse = scale > 0.0F ? __fdiv_rn(1.0F, scale) : 0.0F;
 
     auto store = [&](int row, const uint4& v) {
         const uint32_t words[4] = {v.x, v.y, v.z, v.w};
-        uint32_t codes[2] = {0, 0};
+        uint32_t codes[2];
+        if (finite) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            float x = __uint_as_float(e % 2 == 0 ? words[e / 2] << 16 : words[e / 2] & 0xffff0000U);
-            x = isnan(x) ? 0.0F : x;
-            // an infinity stays one (or becomes NaN at scale 0, which is 0 again)
-            float scaled = __fmul_rn(x, inverse);
-            scaled = isnan(scaled) ? 0.0F : scaled;
-            codes[e / 4] |= encode<INT8>(scaled) << (8 * (e % 4));
+            for (int e = 0; e < 2; ++e) {
+                codes[e] = encode4<INT8>(__fmul_rn(low_bf16(words[2 * e]), inverse), __fmul_rn(high_bf16(words[2 * e]), inverse),
+                                         __fmul_rn(low_bf16(words[2 * e + 1]), inverse), __fmul_rn(high_bf16(words[2 * e + 1]), inverse));
+            }
+        } else {
+            codes[0] = codes[1] = 0;
+            for (int e = 0; e < 8; ++e) {
+                const float x = e % 2 == 0 ? low_bf16(words[e / 2]) : high_bf16(words[e / 2]);
+                codes[e / 4] |= encode_any<INT8>(__fmul_rn(x, inverse)) << (8 * (e % 4));
+            }
         }
         *reinterpret_cast<uint2*>(page + static_cast<size_t>(slot + row) * HEAD + part * 8) = make_uint2(codes[0], codes[1]);
     };
@@ -175,12 +216,12 @@ __global__ void __launch_bounds__(THREADS) flash_cache_append_kernel(const __gri
             uint32_t words[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                uint32_t moved = 0;
+                float x[4];
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    moved |= encode<INT8>(__fmul_rn(decode<INT8>((words[e] >> (8 * k)) & 0xffU), ratio)) << (8 * k);
+                    x[k] = __fmul_rn(decode<INT8>((words[e] >> (8 * k)) & 0xffU), ratio);
                 }
-                words[e] = moved;
+                words[e] = encode4<INT8>(x[0], x[1], x[2], x[3]);
             }
             *at = make_uint4(words[0], words[1], words[2], words[3]);
         }
