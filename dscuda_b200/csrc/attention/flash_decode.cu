@@ -92,10 +92,10 @@ struct DecodeParams {
 template <int SOURCE, int NB>
 struct Shape {
     static constexpr int ROWS = 8 * NB;
-    static constexpr int KEYS = SOURCE == BF16 ? 16 : 32;          // of a warp's step
+    static constexpr int KEYS = SOURCE == BF16 ? 16 : 32;          // of a warp's step (16 with four blocks of rows: 135 us for 123)
     static constexpr int TILE = WARPS * KEYS;
     static constexpr int ROW_BYTES = SOURCE == BF16 ? 256 : 128;
-    static constexpr int OPERAND = KEYS * ROW_BYTES;               // 4 KB
+    static constexpr int OPERAND = KEYS * ROW_BYTES;
     static constexpr int STAGE = 2 * OPERAND;
     static constexpr int CTAS_PER_SM = NB == 1 ? 3 : 2;
     static constexpr int STAGES = NB == 1 ? 2 : 3;
@@ -108,7 +108,7 @@ struct Shape {
 };
 
 struct Scales {
-    float key[2], value[2];             // of the step's two groups of 16 keys
+    float key[2], value[2];             // of the step's one or two groups of 16 keys
 };
 
 __device__ __forceinline__ void copy16(uint32_t dst, const void* src) {
@@ -234,10 +234,10 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
     sm100::grid_dependency_wait();
     // ---- the CTA's range of tiles, and the entry that holds its first one; every warp for itself --------------
     const unsigned items = p.kv_heads * p.row_blocks;
-    unsigned total = 0;
+    unsigned total = 0, own = 0;
     for (int base = 0; base < p.batch; base += 32) {
-        const unsigned cost = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
-        total += __reduce_add_sync(0xffffffffU, cost);
+        own = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
+        total += __reduce_add_sync(0xffffffffU, own);
     }
     const unsigned ctas = min(total, gridDim.x);
     if (blockIdx.x >= ctas) {
@@ -249,7 +249,9 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
     unsigned entry_first = 0;
     int entry = 0;
     for (int base = 0;; base += 32) {
-        const unsigned own = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
+        if (p.batch > 32) {
+            own = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
+        }
         unsigned inclusive = own;
 #pragma unroll
         for (int offset = 1; offset < 32; offset <<= 1) {
@@ -291,7 +293,7 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
         // ---- the warp's keys: steps of KEYS, one to a tile ------------------------------------------------
         const int first_key = tile_begin * S::TILE + warp * KEYS;
         const int steps = min(tile_end - tile_begin, max(0, (length - first_key + S::TILE - 1) / S::TILE));
-        uint32_t place[2] = {0, 0};                     // lane l: where step (s / 32) * 32 + l finds its two groups of 16 keys
+        uint32_t place[KU] = {};                        // lane l: where step (s / 32) * 32 + l finds its groups of 16 keys
         Scales place_scales = {};
         auto issue = [&](int s) {
             if (s < steps) {
@@ -302,7 +304,7 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                         const int key = key0 + lane * S::TILE;
                         if (s + lane < steps) {
 #pragma unroll
-                            for (int u = 0; u < 2; ++u) {
+                            for (int u = 0; u < KU; ++u) {
                                 const int k = min(key + 16 * u, length - 1);
                                 const int logical = k / p.page;
                                 int page = p.table[static_cast<size_t>(entry) * p.pages + logical];
@@ -318,11 +320,8 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                         }
                         __syncwarp();
                     }
-                    if (lane == s % 32) {
-                        scales[warp][s % STAGES] = place_scales;
-                    }
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
+                    for (int u = 0; u < KU; ++u) {
                         const uint32_t at = __shfl_sync(0xffffffffU, place[u], s % 32);
                         const size_t offset = static_cast<size_t>(at) * 128 + lane * 16;        // rows of a group lie one after the other
                         const uint8_t *k = p.keys + offset, *v = p.values + offset;
@@ -343,6 +342,9 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                                 copy16_if(to + S::OPERAND, valid ? v + i * 512 : p.values, valid);
                             }
                         }
+                    }
+                    if (lane == s % 32) {
+                        scales[warp][s % STAGES] = place_scales;        // (behind the copies, which need not wait for them)
                     }
                 } else {
                     const size_t pitch = static_cast<size_t>(p.kv_heads) * 256;
@@ -513,7 +515,7 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
             } else {
                 const Scales meta = scales[warp][s % STAGES];
                 // (a group of keys behind the end repeats the scales of the last one)
-                const float largest = fmaxf(meta.value[0], meta.value[1]);
+                const float largest = fmaxf(meta.value[0], meta.value[KU - 1]);
                 if (largest > unit) {
                     shrink = unit / largest;
                     unit = largest;
