@@ -6,13 +6,15 @@
 // dK and dV of a key head are sums over all rows of its group, so the heads of a group need no step of their own.
 //
 // One call launches:
-//   1. cross_delta_kernel: delta and lse * log2(e) in row order, one pair to a row.
-//   2. cross_query_kernel: a CTA keeps 128 rows and goes over the keys in tiles of 128: S = Q K^T, dP = dO V^T, dQ += dS K.  With few keys the
-//      rounding of O in delta would be the largest error of dS (2 keys: 0.4 % of dQ and dK, against 0.17 % of the last rounding); where one tile
-//      holds all keys, delta = sum_k P dP is formed from the tile itself and left for the next kernel as well.
-//   3. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
+//   1. cross_query_kernel: a CTA keeps 128 rows (Q, dO) and goes over the keys in tiles of 128: S = Q K^T, dP = dO V^T, dQ += dS K.  It forms delta from the
+//      O rows first, and leaves lse * log2(e) and delta in row order for the next kernel.  With few keys the rounding of O in delta would be the largest error
+//      of dS (2 keys: 0.4 % of dQ and dK, against 0.17 % of the last rounding); where one tile holds all keys, delta = sum_k P dP is formed
+//      from the tile itself.
+//   2. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
 //      key (two, half the rows each), P^T and dS^T back into tensor memory as bf16 A operands, dV += P^T dO, dK += dS^T Q.  Tensor memory: dV 128, dK
 //      128, two pairs of 64-column scores, so the scores of the next tile are computed while the softmax works on this one.
+//   3. cross_reduce_kernel, where a grid of whole loops would leave SMs idle: the loops of the first two are cut into parts, whose fp32
+//      sums it adds in order.
 // S and dP are computed twice (1792 instead of 1280 FLOP per pair).  The alternative of the causal backward, dS stored once and streamed
 // back, moves 4 bytes per pair through HBM, 0.62 ps at the measured copy rate, against 0.31 ps for the 512 FLOP at the measured tensor rate.
 //
@@ -26,6 +28,7 @@
 #include "cuda_common.h"
 #include "attention_internal.h"
 #include "sm100_primitives.cuh"
+#include "loop_parts.cuh"
 #include "../common/launch.h"
 #include "../common/tensor_map.h"
 
@@ -50,64 +53,31 @@ constexpr int MMA_WARP = 8;
 constexpr int LOAD_WARP = 9;
 constexpr int TMEM_COLUMNS = 512;
 constexpr float LOG2E = 1.4426950408889634F;
+constexpr int MIN_QUERY_PART = 4;           // key tiles of a part of the query kernel's loop
+constexpr int MIN_KEY_PART = 8;             // row tiles of a part of the key kernel's loop
 
 __device__ int cross_backward_status = 0;
 
 struct CrossBackwardParams {
     CUtensorMap q_sub, do_sub;          // group rows, box {64, group, tokens of a 64-row tile}
-    CUtensorMap q_big, do_big;          // the same for 128-row tiles
+    CUtensorMap q_big, do_big, o_big;   // the same for 128-row tiles
     CUtensorMap k, v;                   // [B][Tk][Hkv * 128], boxes of 128 rows
     CUtensorMap dq;                     // like q_big
     CUtensorMap dk, dv;                 // like k
     float2* rows;                       // [B, Hkv, Tq, group]: lse * log2(e), delta
+    const float* lse;                   // [B, Hq, Tq]
     const int* lengths;                 // null: Tk
-    int tokens, keys, kv_heads, group;
+    float* dq_parts;                    // [query_parts][B, Tq, Hq, 128], where there are several
+    float* dk_parts;                    // [key_parts][B, Tk, Hkv, 128]
+    float* dv_parts;
+    int query_parts, key_parts;
+    int batch, tokens, keys, kv_heads, group;
     int sub_tokens, big_tokens;         // tokens of a query tile of each kind
     float scale, scale_log2;
 };
 
 __device__ __forceinline__ int length_of(const CrossBackwardParams& p, int entry) {
     return p.lengths == nullptr ? p.keys : min(max(p.lengths[entry], 0), p.keys);
-}
-
-// ---------------------------------------------------------------------------
-// delta and lse * log2(e) in row order; half a warp to a row
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(256) cross_delta_kernel(float2* rows, const __nv_bfloat16* dout, const __nv_bfloat16* out, const float* lse,
-                                                          long long count, int tokens, int heads, int group) {
-    const int lane = threadIdx.x % 32;
-    const int half = lane / 16;
-    const int part = lane % 16;
-    const long long stride = static_cast<long long>(gridDim.x) * 16;
-    grid_dependency_wait();
-    for (long long base = static_cast<long long>(blockIdx.x) * 16 + threadIdx.x / 32 * 2; base < count; base += stride) {
-        const long long row = base + half;              // (entry, token, head)
-        float sum = 0.0F;
-        if (row < count) {
-            const uint4 a = reinterpret_cast<const uint4*>(dout + row * HEAD)[part];
-            const uint4 b = reinterpret_cast<const uint4*>(out + row * HEAD)[part];
-            const __nv_bfloat162* a2 = reinterpret_cast<const __nv_bfloat162*>(&a);
-            const __nv_bfloat162* b2 = reinterpret_cast<const __nv_bfloat162*>(&b);
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float2 x = __bfloat1622float2(a2[e]), y = __bfloat1622float2(b2[e]);
-                sum += x.x * y.x + x.y * y.y;
-            }
-        }
-#pragma unroll
-        for (int offset = 8; offset > 0; offset >>= 1) {
-            sum += __shfl_xor_sync(0xffffffffU, sum, offset);
-        }
-        if (part == 0 && row < count) {
-            const int head = static_cast<int>(row % heads);
-            const long long at = row / heads;
-            const long long entry = at / tokens;
-            const int token = static_cast<int>(at % tokens);
-            const int kv_heads = heads / group;
-            rows[((entry * kv_heads + head / group) * tokens + token) * group + head % group] =
-                make_float2(lse[(entry * heads + head) * tokens + token] * LOG2E, sum);
-        }
-    }
 }
 
 // Output tiles leave through idle shared memory: thread r lays out its row of 32 columns in the 128-byte-swizzled chunk that a TMA store reads.
@@ -163,7 +133,9 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
     }
     const int entry = blockIdx.z;
     const int kv_head = blockIdx.y;
-    const int key_start = blockIdx.x * BIG;
+    const int key_tiles = (p.keys + BIG - 1) / BIG;
+    const int part = blockIdx.x / key_tiles;
+    const int key_start = (blockIdx.x - part * key_tiles) * BIG;
     const int rows_per_tile = p.sub_tokens * p.group;
 
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023U) & ~1023U;
@@ -211,7 +183,9 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
     const int length = length_of(p, entry);
     // keys behind the length have gradients of zero: no tiles for them
-    const int tile_count = key_start < length ? (p.tokens + p.sub_tokens - 1) / p.sub_tokens : 0;
+    const int all_tiles = (p.tokens + p.sub_tokens - 1) / p.sub_tokens;
+    const int first_tile = part_begin(all_tiles, part, p.key_parts);
+    const int tile_count = key_start < length ? part_begin(all_tiles, part + 1, p.key_parts) - first_tile : 0;
 
     if (warp == LOAD_WARP) {
         if (tile_count > 0 && lane == 0) {
@@ -233,7 +207,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
                     break;
                 }
             }
-            const int token = t * p.sub_tokens;
+            const int token = (first_tile + t) * p.sub_tokens;
             const uint32_t full = smem_u32(&bars->stage_full[stage]);
             if (lane == 0) {
                 mbar_arrive_expect_tx(full, 4 * rows_per_tile * 128);
@@ -396,23 +370,38 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
             tc_fence_after_sync();
             const bool keep = key_start + r < length;
             uint8_t* stage = smem + (group == 0 ? 2 * BIG_CHUNK : 0);
+            if (p.key_parts > 1) {
+                // keys behind the length are the reduce kernel's zeros
+                float* parts = (group == 0 ? p.dv_parts : p.dk_parts) + static_cast<size_t>(part) * p.batch * p.keys * p.kv_heads * HEAD;
+                const int key0 = key_start + (warp % 4) * 32;
 #pragma unroll
-            for (int c = 0; c < HEAD / 32; ++c) {
-                uint32_t values[32];
-                if (tile_count > 0) {
+                for (int c = 0; c < HEAD / 32 && tile_count > 0; ++c) {
+                    uint32_t values[32];
                     tmem_ld_x32(tmem_base + lane_base + (group == 0 ? TMEM_DV : TMEM_DK) + c * 32, values);
                     tmem_wait_ld();
+                    store_f32_rows(stage + (warp % 4) * 4096, lane, values, [&](int row) -> float* {
+                        return key0 + row < length ? parts + ((static_cast<size_t>(entry) * p.keys + key0 + row) * p.kv_heads + kv_head) * HEAD + c * 32 : nullptr;
+                    });
                 }
-                stage_bf16x32(stage + (c / 2) * BIG_CHUNK, r, c % 2, values, keep && tile_count > 0);
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(smem_u32(&bars->staged[group]));
-            if (r == 0 && mbar_wait(smem_u32(&bars->staged[group]), 0, abort_flag, &cross_backward_status)) {
-                for (int c = 0; c < 2; ++c) {
-                    tma_store_3d(group == 0 ? &p.dv : &p.dk, (group == 0 ? v_smem : k_smem) + c * BIG_CHUNK, kv_head * HEAD + c * 64, key_start, entry);
+            } else {
+#pragma unroll
+                for (int c = 0; c < HEAD / 32; ++c) {
+                    uint32_t values[32];
+                    if (tile_count > 0) {
+                        tmem_ld_x32(tmem_base + lane_base + (group == 0 ? TMEM_DV : TMEM_DK) + c * 32, values);
+                        tmem_wait_ld();
+                    }
+                    stage_bf16x32(stage + (c / 2) * BIG_CHUNK, r, c % 2, values, keep && tile_count > 0);
                 }
-                tma_store_commit();
-                tma_store_wait_read();
+                fence_proxy_async_smem();
+                mbar_arrive(smem_u32(&bars->staged[group]));
+                if (r == 0 && mbar_wait(smem_u32(&bars->staged[group]), 0, abort_flag, &cross_backward_status)) {
+                    for (int c = 0; c < 2; ++c) {
+                        tma_store_3d(group == 0 ? &p.dv : &p.dk, (group == 0 ? v_smem : k_smem) + c * BIG_CHUNK, kv_head * HEAD + c * 64, key_start, entry);
+                    }
+                    tma_store_commit();
+                    tma_store_wait_read();
+                }
             }
         }
     }
@@ -433,15 +422,15 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
 
 // ---------------------------------------------------------------------------
 // dQ: 128 rows resident (Q in shared memory, dO in tensor memory), tiles of 128 keys.  Order of the tensor core: S(j+1) | dQ(j) | dP(j+1).
-// K(j) is read by S(j) and again by dQ(j), a tile and a half later: three slots; V in two.
+// K(j) is read by S(j) and again by dQ(j), a tile and a half later: three slots, the last of which first holds O; V in two, the second of which first holds dO.
 // ---------------------------------------------------------------------------
 namespace queryside {
 constexpr int KEYS = 128;
 constexpr int Q_BYTES = 2 * BIG_CHUNK;
 constexpr int TILE_BYTES = 2 * BIG_CHUNK;
 constexpr int K_SLOTS = 3;
-constexpr int V_SLOTS = 2;                          // the second one first holds dO
-constexpr int MISC_BYTES = 2048;
+constexpr int V_SLOTS = 2;
+constexpr int MISC_BYTES = 3072;
 constexpr int SMEM_BYTES = Q_BYTES + (K_SLOTS + V_SLOTS) * TILE_BYTES + MISC_BYTES + 1024;
 constexpr uint32_t TMEM_S = 0;
 constexpr uint32_t TMEM_DP = 128;
@@ -465,7 +454,7 @@ struct Barriers {
     uint64_t delta_full;
     uint32_t tmem_base;
     int abort_flag;
-    float delta[2][BIG];        // one key tile: each half's share of sum_k P dP
+    float delta[2][2][BIG];     // each half's share of sum_d dO O, and with one key tile of sum_k P dP
 };
 static_assert(sizeof(Barriers) <= MISC_BYTES, "barrier block too large");
 }  // namespace queryside
@@ -479,7 +468,9 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
     }
     const int entry = blockIdx.z;
     const int kv_head = blockIdx.y;
-    const int token0 = blockIdx.x * p.big_tokens;
+    const int row_tiles = (p.tokens + p.big_tokens - 1) / p.big_tokens;
+    const int part = blockIdx.x / row_tiles;
+    const int token0 = (blockIdx.x - part * row_tiles) * p.big_tokens;
     const int rows_per_tile = p.big_tokens * p.group;
 
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023U) & ~1023U;
@@ -524,12 +515,15 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
     grid_dependency_wait();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
     const int length = length_of(p, entry);
-    const int tile_count = (length + KEYS - 1) / KEYS;
+    const int all_tiles = (length + KEYS - 1) / KEYS;
+    const int first_tile = part_begin(all_tiles, part, p.query_parts);
+    const int tile_count = part_begin(all_tiles, part + 1, p.query_parts) - first_tile;
+    const int left = length - first_tile * KEYS;        // keys from the first tile on
 
     if (warp == LOAD_WARP) {
         if (tile_count > 0) {
             const int last = tile_count - 1;
-            const bool ragged = length < p.keys && tile_count * KEYS > length;
+            const bool ragged = length < p.keys && tile_count * KEYS > left;
             bool alive = true;
             auto load_v = [&](int j) {
                 const int slot = j % V_SLOTS;
@@ -544,12 +538,14 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                 const uint32_t full = smem_u32(ragged && j == last ? &bars->tail_full[1] : &bars->v_full[slot]);
                 mbar_arrive_expect_tx(full, TILE_BYTES);
                 for (int c = 0; c < 2; ++c) {
-                    tma_load_3d(v_ring + slot * TILE_BYTES + c * BIG_CHUNK, &p.v, full, kv_head * HEAD + c * 64, j * KEYS, entry);
+                    tma_load_3d(v_ring + slot * TILE_BYTES + c * BIG_CHUNK, &p.v, full, kv_head * HEAD + c * 64, (first_tile + j) * KEYS, entry);
                 }
             };
             auto load_k = [&](int j) {
                 const int slot = j % K_SLOTS;
-                if (j >= K_SLOTS) {
+                if (j == K_SLOTS - 1) {
+                    alive = mbar_wait(smem_u32(&bars->do_copied), 0, abort_flag, &cross_backward_status);
+                } else if (j >= K_SLOTS) {
                     alive = mbar_wait(smem_u32(&bars->k_empty[slot]), (j / K_SLOTS - 1) & 1, abort_flag, &cross_backward_status);
                 }
                 if (!alive) {
@@ -558,7 +554,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                 const uint32_t full = smem_u32(ragged && j == last ? &bars->tail_full[0] : &bars->k_full[slot]);
                 mbar_arrive_expect_tx(full, TILE_BYTES);
                 for (int c = 0; c < 2; ++c) {
-                    tma_load_3d(k_ring + slot * TILE_BYTES + c * BIG_CHUNK, &p.k, full, kv_head * HEAD + c * 64, j * KEYS, entry);
+                    tma_load_3d(k_ring + slot * TILE_BYTES + c * BIG_CHUNK, &p.k, full, kv_head * HEAD + c * 64, (first_tile + j) * KEYS, entry);
                 }
             };
             auto clear_tail = [&](int which, uint32_t offset, uint64_t* full) {
@@ -568,7 +564,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                     return;
                 }
                 for (int c = 0; c < 2; ++c) {
-                    clear_rows(smem + offset + c * BIG_CHUNK, length - last * KEYS, KEYS, lane);
+                    clear_rows(smem + offset + c * BIG_CHUNK, left - last * KEYS, KEYS, lane);
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
@@ -578,9 +574,10 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
             };
             if (lane == 0) {
                 const uint32_t bar = smem_u32(&bars->resident_full);
-                mbar_arrive_expect_tx(bar, 4 * rows_per_tile * 128);
+                mbar_arrive_expect_tx(bar, 6 * rows_per_tile * 128);
                 for (int c = 0; c < 2; ++c) {
                     tma_load_4d(smem_base + c * BIG_CHUNK, &p.q_big, bar, c * 64, kv_head * p.group, token0, entry);
+                    tma_load_4d(k_ring + (K_SLOTS - 1) * TILE_BYTES + c * BIG_CHUNK, &p.o_big, bar, c * 64, kv_head * p.group, token0, entry);
                     tma_load_4d(v_ring + TILE_BYTES + c * BIG_CHUNK, &p.do_big, bar, c * 64, kv_head * p.group, token0, entry);
                 }
                 for (int j = 0; j < tile_count && alive; ++j) {
@@ -689,13 +686,11 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
         const uint32_t lane_base = static_cast<uint32_t>((warp % 4) * 32) << 16;
         const int token = token0 + r / p.group;
         const bool valid = r < rows_per_tile && token < p.tokens;
-        const size_t row_index = ((static_cast<size_t>(entry) * p.kv_heads + kv_head) * p.tokens + token) * p.group + r % p.group;
-        float2 constants = make_float2(INFINITY, 0.0F);
+        float lse2 = INFINITY;
         if (valid) {
-            constants = p.rows[row_index];
+            lse2 = p.lse[(static_cast<size_t>(entry) * p.kv_heads * p.group + kv_head * p.group + r % p.group) * p.tokens + token] * LOG2E;
         }
-        const float lse2 = constants.x;
-        float delta = constants.y;
+        float delta = 0.0F;
         bool alive = true;
         if (tile_count > 0) {
             alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->resident_full), 0, abort_flag, &cross_backward_status));
@@ -712,10 +707,32 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                     values[unit * 4 + 3] = v.w;
                 }
                 tmem_st_x32(tmem_base + lane_base + TMEM_DO + half * 32, values);
+                const uint8_t* out = smem + Q_BYTES + (K_SLOTS - 1) * TILE_BYTES + half * BIG_CHUNK + r * 128;
+                float share = 0.0F;
+#pragma unroll
+                for (int unit = 0; unit < 8; ++unit) {
+                    const uint4 v = *reinterpret_cast<const uint4*>(out + ((unit ^ (r & 7)) * 16));
+                    const uint32_t words[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        share = fmaf(__uint_as_float(values[unit * 4 + e] << 16), __uint_as_float(words[e] << 16), share);
+                        share = fmaf(__uint_as_float(values[unit * 4 + e] & 0xffff0000U), __uint_as_float(words[e] & 0xffff0000U), share);
+                    }
+                }
+                bars->delta[0][half][r] = share;
                 tmem_wait_st();
                 tc_fence_before_sync();
                 mbar_arrive(smem_u32(&bars->do_copied));
+                alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->do_copied), 0, abort_flag, &cross_backward_status));
+                delta = bars->delta[0][0][r] + bars->delta[0][1][r];
             }
+        }
+        // (the last part always has a tile of an entry that has any)
+        float2* row = valid && half == 0 && part + 1 == p.query_parts && length > 0
+                          ? p.rows + ((static_cast<size_t>(entry) * p.kv_heads + kv_head) * p.tokens + token) * p.group + r % p.group
+                          : nullptr;
+        if (row != nullptr && alive) {
+            *row = make_float2(lse2, delta);
         }
         const uint32_t s_tmem = tmem_base + lane_base + TMEM_S + half * 64;
         const uint32_t dp_tmem = tmem_base + lane_base + TMEM_DP + half * 64;
@@ -737,10 +754,10 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                 prob[n] = exp2_approx(fmaf(__uint_as_float(sb[n]), p.scale_log2, -lse2)) * p.scale;
             }
             if (j + 1 == tile_count) {
-                const int left = length - j * KEYS - half * 64;
+                const int present = left - j * KEYS - half * 64;
 #pragma unroll
                 for (int n = 0; n < 64; ++n) {
-                    prob[n] = n < left ? prob[n] : 0.0F;
+                    prob[n] = n < present ? prob[n] : 0.0F;
                 }
             }
             alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->dp_full), j & 1, abort_flag, &cross_backward_status));
@@ -751,21 +768,21 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
             tmem_ld_x32(dp_tmem, sb);
             tmem_ld_x32(dp_tmem + 32, sb + 32);
             tmem_wait_ld();
-            if (tile_count == 1) {
+            if (all_tiles == 1) {
                 float share = 0.0F;
 #pragma unroll
                 for (int n = 0; n < 64; ++n) {
                     share = fmaf(prob[n], __uint_as_float(sb[n]), share);
                 }
-                bars->delta[half][r] = share;
+                bars->delta[1][half][r] = share;
                 mbar_arrive(smem_u32(&bars->delta_full));
                 alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->delta_full), 0, abort_flag, &cross_backward_status));
                 if (!alive) {
                     break;
                 }
-                delta = (bars->delta[0][r] + bars->delta[1][r]) / p.scale;
-                if (valid && half == 0) {
-                    p.rows[row_index].y = delta;
+                delta = (bars->delta[1][0][r] + bars->delta[1][1][r]) / p.scale;
+                if (row != nullptr) {
+                    row->y = delta;
                 }
             }
             uint32_t packed[32];
@@ -783,23 +800,40 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
         }
         if (alive) {
             tc_fence_after_sync();
+            if (p.query_parts > 1) {
+                float* parts = p.dq_parts + static_cast<size_t>(part) * p.batch * p.tokens * p.kv_heads * p.group * HEAD;
 #pragma unroll
-            for (int c = 0; c < 2; ++c) {
-                uint32_t values[32];
-                if (tile_count > 0) {
+                for (int c = 0; c < 2 && tile_count > 0; ++c) {
+                    uint32_t values[32];
                     tmem_ld_x32(tmem_base + lane_base + TMEM_DQ + half * 64 + c * 32, values);
                     tmem_wait_ld();
+                    store_f32_rows(smem + warp * 4096, lane, values, [&](int index) -> float* {
+                        const int at = (warp % 4) * 32 + index;
+                        const int t = token0 + at / p.group;
+                        return at < rows_per_tile && t < p.tokens
+                                   ? parts + ((static_cast<size_t>(entry) * p.tokens + t) * p.kv_heads * p.group + kv_head * p.group + at % p.group) * HEAD + half * 64 + c * 32
+                                   : nullptr;
+                    });
                 }
-                stage_bf16x32(smem + half * BIG_CHUNK, r, c, values, tile_count > 0);
-            }
-            fence_proxy_async_smem();
-            mbar_arrive(smem_u32(&bars->staged));
-            if (threadIdx.x == 0 && mbar_wait(smem_u32(&bars->staged), 0, abort_flag, &cross_backward_status)) {
+            } else {
+#pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    tma_store_4d(&p.dq, smem_base + c * BIG_CHUNK, c * 64, kv_head * p.group, token0, entry);
+                    uint32_t values[32];
+                    if (tile_count > 0) {
+                        tmem_ld_x32(tmem_base + lane_base + TMEM_DQ + half * 64 + c * 32, values);
+                        tmem_wait_ld();
+                    }
+                    stage_bf16x32(smem + half * BIG_CHUNK, r, c, values, tile_count > 0);
                 }
-                tma_store_commit();
-                tma_store_wait_read();
+                fence_proxy_async_smem();
+                mbar_arrive(smem_u32(&bars->staged));
+                if (threadIdx.x == 0 && mbar_wait(smem_u32(&bars->staged), 0, abort_flag, &cross_backward_status)) {
+                    for (int c = 0; c < 2; ++c) {
+                        tma_store_4d(&p.dq, smem_base + c * BIG_CHUNK, c * 64, kv_head * p.group, token0, entry);
+                    }
+                    tma_store_commit();
+                    tma_store_wait_read();
+                }
             }
         }
     }
@@ -816,6 +850,80 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, TMEM_COLUMNS);
     }
+}
+
+// ---------------------------------------------------------------------------
+// Parts added in order; a thread takes four columns of a row
+// ---------------------------------------------------------------------------
+__device__ __forceinline__ uint2 sum_parts(const float* parts, size_t offset, size_t stride, int first, int last) {
+    float4 sum = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+#pragma unroll 4
+    for (int part = first; part < last; ++part) {
+        const float4 x = *reinterpret_cast<const float4*>(parts + part * stride + offset);
+        sum.x += x.x;
+        sum.y += x.y;
+        sum.z += x.z;
+        sum.w += x.w;
+    }
+    return make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+}
+
+__global__ void __launch_bounds__(256) cross_reduce_kernel(const __grid_constant__ CrossBackwardParams p, uint2* dq, uint2* dk, uint2* dv) {
+    const size_t entry_query = static_cast<size_t>(p.tokens) * p.kv_heads * p.group * (HEAD / 4);       // units of an entry
+    const size_t entry_key = static_cast<size_t>(p.keys) * p.kv_heads * (HEAD / 4);
+    const size_t queries = p.query_parts > 1 ? p.batch * entry_query : 0;
+    const size_t keys = p.key_parts > 1 ? p.batch * entry_key : 0;
+    const size_t step = static_cast<size_t>(gridDim.x) * 256;
+    grid_dependency_wait();
+    for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < queries + keys; i += step) {
+        if (i < queries) {
+            // a part without tiles has written nothing
+            const int tiles = (length_of(p, static_cast<int>(i / entry_query)) + queryside::KEYS - 1) / queryside::KEYS;
+            uint2 result = make_uint2(0, 0);
+            if (tiles >= p.query_parts) {
+                result = sum_parts(p.dq_parts, i * 4, p.batch * entry_query * 4, 0, p.query_parts);
+            } else {
+                float4 sum = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+                for (int part = 0; part < p.query_parts; ++part) {
+                    if (part_begin(tiles, part, p.query_parts) < part_begin(tiles, part + 1, p.query_parts)) {
+                        const float4 x = *reinterpret_cast<const float4*>(p.dq_parts + part * (p.batch * entry_query * 4) + i * 4);
+                        sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+                    }
+                }
+                result = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
+            }
+            dq[i] = result;
+        } else {
+            const size_t at = i - queries;
+            const int entry = static_cast<int>(at / entry_key);
+            const int key = static_cast<int>((at - entry * entry_key) / (p.kv_heads * (HEAD / 4)));
+            const bool present = key < length_of(p, entry);
+            dk[at] = present ? sum_parts(p.dk_parts, at * 4, keys * 4, 0, p.key_parts) : make_uint2(0, 0);
+            dv[at] = present ? sum_parts(p.dv_parts, at * 4, keys * 4, 0, p.key_parts) : make_uint2(0, 0);
+        }
+    }
+}
+
+struct Plan {
+    int query_parts, key_parts;
+    std::size_t rows_bytes, query_bytes, key_bytes;         // of the row constants, of all parts of dQ, of all parts of dK (and dV)
+    std::size_t bytes() const { return rows_bytes + query_bytes + 2 * key_bytes; }
+};
+
+Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
+    const int group = heads / kv_heads;
+    const long long key_tiles = (keys + BIG - 1LL) / BIG;
+    const long long row_tiles = (queries + BIG / group - 1LL) / (BIG / group);
+    const long long sub_tiles = (queries + SUB / group - 1LL) / (SUB / group);
+    const long long pairs = static_cast<long long>(batch) * kv_heads;
+    Plan plan{};
+    plan.query_parts = loop_parts(row_tiles * pairs, key_tiles, MIN_QUERY_PART);
+    plan.key_parts = loop_parts(key_tiles * pairs, sub_tiles, MIN_KEY_PART);
+    const std::size_t query_rows = static_cast<std::size_t>(batch) * queries * heads, key_rows = static_cast<std::size_t>(batch) * keys * kv_heads;
+    plan.rows_bytes = (query_rows * sizeof(float2) + 15) / 16 * 16;
+    plan.query_bytes = plan.query_parts > 1 ? plan.query_parts * query_rows * HEAD * sizeof(float) : 0;
+    plan.key_bytes = plan.key_parts > 1 ? plan.key_parts * key_rows * HEAD * sizeof(float) : 0;
+    return plan;
 }
 
 void configure() {
@@ -853,7 +961,10 @@ std::size_t flash_cross_backward_workspace_bytes(int batch_size, int query_lengt
     if (batch_size <= 0 || query_length <= 0 || key_length <= 0 || query_heads <= 0 || key_value_heads <= 0) {
         return 0;
     }
-    return static_cast<std::size_t>(batch_size) * query_length * query_heads * sizeof(float2);
+    if (query_heads % key_value_heads != 0 || query_heads / key_value_heads > SUB) {
+        return 0;                   // refused by the call
+    }
+    return make_plan(batch_size, query_length, key_length, query_heads, key_value_heads).bytes();
 }
 
 void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key_gradient, __nv_bfloat16* value_gradient,
@@ -878,26 +989,39 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     p.do_sub = make_bf16_group_rows_map(output_gradient, batch_size, query_length, query_heads, p.group, p.sub_tokens);
     p.q_big = make_bf16_group_rows_map(query, batch_size, query_length, query_heads, p.group, p.big_tokens);
     p.do_big = make_bf16_group_rows_map(output_gradient, batch_size, query_length, query_heads, p.group, p.big_tokens);
+    p.o_big = make_bf16_group_rows_map(output, batch_size, query_length, query_heads, p.group, p.big_tokens);
     p.dq = make_bf16_group_rows_map(query_gradient, batch_size, query_length, query_heads, p.group, p.big_tokens);
     p.k = make_bf16_batched_tile_map(key, batch_size, key_length, wide, BIG);
     p.v = make_bf16_batched_tile_map(value, batch_size, key_length, wide, BIG);
     p.dk = make_bf16_batched_tile_map(key_gradient, batch_size, key_length, wide, BIG);
     p.dv = make_bf16_batched_tile_map(value_gradient, batch_size, key_length, wide, BIG);
-    p.rows = static_cast<float2*>(workspace);
+    const Plan plan = make_plan(batch_size, query_length, key_length, query_heads, key_value_heads);
+    uint8_t* memory = static_cast<uint8_t*>(workspace);
+    p.rows = reinterpret_cast<float2*>(memory);
+    p.dq_parts = reinterpret_cast<float*>(memory + plan.rows_bytes);
+    p.dk_parts = reinterpret_cast<float*>(memory + plan.rows_bytes + plan.query_bytes);
+    p.dv_parts = reinterpret_cast<float*>(memory + plan.rows_bytes + plan.query_bytes + plan.key_bytes);
+    p.query_parts = plan.query_parts;
+    p.key_parts = plan.key_parts;
+    p.lse = logsumexp;
     p.lengths = key_lengths;
+    p.batch = batch_size;
     p.tokens = query_length;
     p.keys = key_length;
     p.kv_heads = key_value_heads;
     p.scale = scale;
     p.scale_log2 = scale * LOG2E;
     configure();
-    const long long rows = static_cast<long long>(batch_size) * query_length * query_heads;
-    const unsigned blocks = static_cast<unsigned>(std::min((rows + 15) / 16, 148LL * 16));
-    launch_chained(cross_delta_kernel, dim3(blocks), dim3(256), 0, stream, static_cast<float2*>(workspace), output_gradient, output, logsumexp, rows,
-                   query_length, query_heads, p.group);
-    launch_chained(cross_query_kernel, dim3((query_length + p.big_tokens - 1) / p.big_tokens, key_value_heads, batch_size), dim3(THREADS),
+    launch_chained(cross_query_kernel, dim3((query_length + p.big_tokens - 1) / p.big_tokens * plan.query_parts, key_value_heads, batch_size), dim3(THREADS),
                    queryside::SMEM_BYTES, stream, p);
-    launch_chained(cross_key_kernel, dim3((key_length + BIG - 1) / BIG, key_value_heads, batch_size), dim3(THREADS), keyside::SMEM_BYTES, stream, p);
+    launch_chained(cross_key_kernel, dim3((key_length + BIG - 1) / BIG * plan.key_parts, key_value_heads, batch_size), dim3(THREADS), keyside::SMEM_BYTES,
+                   stream, p);
+    if (plan.query_parts > 1 || plan.key_parts > 1) {
+        const long long units = ((plan.query_parts > 1 ? static_cast<long long>(batch_size) * query_length * query_heads : 0) +
+                                 (plan.key_parts > 1 ? static_cast<long long>(batch_size) * key_length * key_value_heads : 0)) * (HEAD / 4);
+        launch_chained(cross_reduce_kernel, dim3(static_cast<unsigned>(std::min((units + 255) / 256, SMS * 8))), dim3(256), 0, stream, p,
+                       reinterpret_cast<uint2*>(query_gradient), reinterpret_cast<uint2*>(key_gradient), reinterpret_cast<uint2*>(value_gradient));
+    }
 }
 
 }  // namespace dscuda

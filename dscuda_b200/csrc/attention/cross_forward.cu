@@ -11,6 +11,9 @@
 // entry's length (a weight of zero does not keep their NaN out of P V) and complete the third warpgroup, which hands registers to the
 // softmax.  The schedule is that of prefill_forward.cu, where its measurements stand.
 //
+// Small problems: where pairs of tiles would leave SMs idle a CTA takes one tile, and where that is not enough the loop over the keys is cut into parts,
+// whose fp32 results cross_combine_kernel joins.
+//
 // Few rows to a key head (single tokens) go to flash_decode.cu instead, which splits the keys over the SMs.
 //
 // P is rounded to bf16 (half a step is 2^-9 of each weight); sums, maxima and O are fp32.  Every wait is bounded.
@@ -18,6 +21,7 @@
 #include "cuda_common.h"
 #include "attention_internal.h"
 #include "sm100_primitives.cuh"
+#include "loop_parts.cuh"
 #include "../common/launch.h"
 #include "../common/tensor_map.h"
 
@@ -53,8 +57,12 @@ struct CrossForwardParams {
     CUtensorMap out;            // like q
     float* lse;                 // [B, Hq, Tq]
     const int* lengths;         // null: Tk
-    int tokens, keys, heads, group;
+    float* part_out;            // [parts][B, Tq, Hq, 128], where there are several
+    float* part_lse;            // [parts][B, Hq, Tq], log2 domain
+    int batch, tokens, keys, heads, group;
     int tile_tokens;            // tokens of a query tile
+    int cta_tiles;              // query tiles of a CTA: 1 or 2
+    int parts;                  // CTAs that share the keys of a query tile
     float scale, scale_log2;
 };
 
@@ -81,8 +89,10 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
     const int entry = blockIdx.z;
     const int kv_head = blockIdx.y;
     const int row_tiles = (p.tokens + p.tile_tokens - 1) / p.tile_tokens;
-    const int tile0 = blockIdx.x * 2;
-    const bool second = tile0 + 1 < row_tiles;
+    const int row_ctas = (row_tiles + p.cta_tiles - 1) / p.cta_tiles;
+    const int part = blockIdx.x / row_ctas;
+    const int tile0 = (blockIdx.x - part * row_ctas) * p.cta_tiles;
+    const bool second = p.cta_tiles == 2 && tile0 + 1 < row_tiles;
 
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023U) & ~1023U;
     uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
@@ -123,9 +133,12 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
     grid_dependency_wait();
     const uint32_t tmem_base = *reinterpret_cast<volatile uint32_t*>(&bars->tmem_base);
     const int length = p.lengths == nullptr ? p.keys : min(max(p.lengths[entry], 0), p.keys);
-    const int tile_count = (length + TILE - 1) / TILE;
+    const int all_tiles = (length + TILE - 1) / TILE;
+    const int first_tile = part_begin(all_tiles, part, p.parts);
+    const int tile_count = part_begin(all_tiles, part + 1, p.parts) - first_tile;
+    const int left = length - first_tile * TILE;        // keys from the first tile on
     // what lies between the length and the end of the entry's states may be anything; behind that end the loads give zeros
-    const int tail_keys = length < p.keys ? length - (tile_count - 1) * TILE : TILE;
+    const int tail_keys = length < p.keys ? min(left - (tile_count - 1) * TILE, TILE) : TILE;
 
     constexpr int REG_LO = 88;
     constexpr int REG_HI = 208;
@@ -180,7 +193,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
                         uint32_t bar;
                         const uint32_t dst = acquire(bar, nullptr);
                         if (dst != 0) {
-                            tma_load_3d(dst, &p.k, bar, kv_head * HEAD + c * 64, j * TILE, entry);
+                            tma_load_3d(dst, &p.k, bar, kv_head * HEAD + c * 64, (first_tile + j) * TILE, entry);
                         }
                     }
                     if (j == 0 && second) {
@@ -191,8 +204,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
                         uint32_t bar;
                         const uint32_t dst = acquire(bar, tail ? &bars->tail_full[half] : nullptr);
                         if (dst != 0) {
-                            tma_load_3d(dst, &p.v, bar, kv_head * HEAD, j * TILE + half * 64, entry);
-                            tma_load_3d(dst + CHUNK / 2, &p.v, bar, kv_head * HEAD + 64, j * TILE + half * 64, entry);
+                            tma_load_3d(dst, &p.v, bar, kv_head * HEAD, (first_tile + j) * TILE + half * 64, entry);
+                            tma_load_3d(dst + CHUNK / 2, &p.v, bar, kv_head * HEAD + 64, (first_tile + j) * TILE + half * 64, entry);
                         }
                     }
                 }
@@ -305,10 +318,10 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
             }
             tmem_wait_ld();
             if (j == count - 1) {
-                const int left = length - j * TILE;
+                const int present = left - j * TILE;
 #pragma unroll
                 for (int n = 0; n < TILE; ++n) {
-                    sb[n] = n < left ? sb[n] : 0xff800000U;
+                    sb[n] = n < present ? sb[n] : 0xff800000U;
                 }
             }
             float mx0 = __uint_as_float(sb[0]), mx1 = __uint_as_float(sb[1]), mx2 = __uint_as_float(sb[2]), mx3 = __uint_as_float(sb[3]);
@@ -377,7 +390,34 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
         if (alive && count > 0) {
             alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->s_full[i]), count & 1, abort_flag, &cross_forward_status));
         }
-        if (alive && active) {
+        if (alive && active && p.parts > 1) {
+            // (a part without tiles has nothing to write)
+            if (count > 0) {
+                tc_fence_after_sync();
+                const float inverse = 1.0F / l_sum;
+                const size_t rows = static_cast<size_t>(p.batch) * p.tokens * p.heads;
+#pragma unroll
+                for (int c = 0; c < HEAD / 32; ++c) {
+                    uint32_t o[32];
+                    tmem_ld_x32(o_tmem + c * 32, o);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int e = 0; e < 32; ++e) {
+                        o[e] = __float_as_uint(__uint_as_float(o[e]) * inverse);
+                    }
+                    store_f32_rows(smem + 2 * i * CHUNK + (warp % 4) * 4096, lane, o, [&](int index) -> float* {
+                        const int at = (warp % 4) * 32 + index;
+                        const int t = (tile0 + i) * p.tile_tokens + at / p.group;
+                        return at < p.tile_tokens * p.group && t < p.tokens
+                                   ? p.part_out + (part * rows + (static_cast<size_t>(entry) * p.tokens + t) * p.heads + kv_head * p.group + at % p.group) * HEAD + c * 32
+                                   : nullptr;
+                    });
+                }
+                if (valid) {
+                    p.part_lse[part * rows + (lse - p.lse)] = m_ref * p.scale_log2 + log2f(l_sum);
+                }
+            }
+        } else if (alive && active) {
             // rows of 64 columns into the tile's Q chunks (idle by now), from where a TMA store takes them
             tc_fence_after_sync();
             const float inverse = count > 0 ? 1.0F / l_sum : 0.0F;
@@ -432,6 +472,65 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
         tc_fence_after_sync();
         tmem_dealloc(tmem_base, TMEM_COLUMNS);
     }
+}
+
+// Joins the parts of every row in the order of their keys; a warp to a row, four columns to a lane.
+__global__ void __launch_bounds__(128) cross_combine_kernel(const __grid_constant__ CrossForwardParams p, uint2* out) {
+    const long long rows = static_cast<long long>(p.batch) * p.tokens * p.heads;
+    const long long row = blockIdx.x * 4LL + threadIdx.x / 32;          // (entry, token, head)
+    const int lane = threadIdx.x % 32;
+    if (row >= rows) {
+        return;
+    }
+    const int head = static_cast<int>(row % p.heads);
+    const long long at = row / p.heads;
+    const int entry = static_cast<int>(at / p.tokens);
+    const long long lse_index = (static_cast<long long>(entry) * p.heads + head) * p.tokens + at % p.tokens;
+    grid_dependency_wait();
+    const int length = p.lengths == nullptr ? p.keys : min(max(p.lengths[entry], 0), p.keys);
+    const int tiles = (length + TILE - 1) / TILE;
+    auto present = [&](int part) { return part_begin(tiles, part, p.parts) < part_begin(tiles, part + 1, p.parts); };
+    float top = -INFINITY;
+    for (int part = 0; part < p.parts; ++part) {
+        top = present(part) ? fmaxf(top, p.part_lse[part * rows + lse_index]) : top;
+    }
+    const float reference = top == -INFINITY ? 0.0F : top;
+    float sum = 0.0F;
+    float4 value = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+    for (int part = 0; part < p.parts; ++part) {
+        if (present(part)) {
+            const float weight = exp2_approx(p.part_lse[part * rows + lse_index] - reference);
+            const float4 x = *reinterpret_cast<const float4*>(p.part_out + (part * rows + row) * HEAD + lane * 4);
+            sum += weight;
+            value = make_float4(value.x + weight * x.x, value.y + weight * x.y, value.z + weight * x.z, value.w + weight * x.w);
+        }
+    }
+    const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
+    out[row * 32 + lane] = make_uint2(pack_bf16x2(value.x * inverse, value.y * inverse), pack_bf16x2(value.z * inverse, value.w * inverse));
+    if (lane == 0) {
+        p.lse[lse_index] = sum == 0.0F ? -INFINITY : (reference + log2f(sum)) * 0.6931471805599453F;
+    }
+}
+
+// How a call's rows and keys are dealt to CTAs.
+constexpr int MIN_PART = 4;                 // key tiles of a part
+
+struct Plan {
+    int cta_tiles, row_ctas, parts;
+    std::size_t rows;
+    std::size_t bytes() const { return parts > 1 ? parts * rows * (HEAD + 1) * sizeof(float) : 0; }
+};
+
+Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
+    const int tile_tokens = TILE / (heads / kv_heads);
+    const long long row_tiles = (queries + tile_tokens - 1LL) / tile_tokens;
+    const long long pairs = static_cast<long long>(batch) * kv_heads;
+    Plan plan{};
+    plan.cta_tiles = row_tiles * pairs <= SMS ? 1 : 2;
+    plan.row_ctas = static_cast<int>((row_tiles + plan.cta_tiles - 1) / plan.cta_tiles);
+    plan.parts = loop_parts(plan.row_ctas * pairs, (keys + TILE - 1LL) / TILE, MIN_PART);
+    plan.rows = static_cast<std::size_t>(batch) * queries * heads;
+    return plan;
 }
 
 void configure() {
@@ -495,7 +594,13 @@ std::size_t flash_cross_forward_workspace_bytes(int batch_size, int query_length
         return 0;
     }
     const long long rows = static_cast<long long>(query_length) * (query_heads / key_value_heads);
-    return rows <= FEW_ROWS ? internal::few_rows_workspace_bytes(batch_size, key_value_heads, rows) : 0;
+    if (rows <= FEW_ROWS) {
+        return internal::few_rows_workspace_bytes(batch_size, key_value_heads, rows);
+    }
+    if (query_heads % key_value_heads != 0 || query_heads / key_value_heads > 64) {
+        return 0;                   // refused by the call
+    }
+    return make_plan(batch_size, query_length, key_length, query_heads, key_value_heads).bytes();
 }
 
 void flash_cross_forward_cuda(__nv_bfloat16* output, float* logsumexp, const __nv_bfloat16* query, const __nv_bfloat16* key,
@@ -534,9 +639,17 @@ void flash_cross_forward_cuda(__nv_bfloat16* output, float* logsumexp, const __n
     p.group = group;
     p.scale = scale;
     p.scale_log2 = scale * LOG2E;
+    const Plan plan = make_plan(batch_size, query_length, key_length, query_heads, key_value_heads);
+    p.batch = batch_size;
+    p.cta_tiles = plan.cta_tiles;
+    p.parts = plan.parts;
+    p.part_out = static_cast<float*>(workspace);
+    p.part_lse = p.part_out + plan.parts * plan.rows * HEAD;
     configure();
-    const int row_tiles = (query_length + p.tile_tokens - 1) / p.tile_tokens;
-    launch_chained(cross_forward_kernel, dim3((row_tiles + 1) / 2, key_value_heads, batch_size), dim3(THREADS), SMEM_BYTES, stream, p);
+    launch_chained(cross_forward_kernel, dim3(plan.row_ctas * plan.parts, key_value_heads, batch_size), dim3(THREADS), SMEM_BYTES, stream, p);
+    if (plan.parts > 1) {
+        launch_chained(cross_combine_kernel, dim3(static_cast<unsigned>((plan.rows + 3) / 4)), dim3(128), 0, stream, p, reinterpret_cast<uint2*>(output));
+    }
 }
 
 }  // namespace dscuda

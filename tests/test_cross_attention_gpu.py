@@ -53,6 +53,8 @@ SHAPES = [
     (1, 1, 1, 1, 1, None), (1, 33, 1, 1, 1, None), (2, 1, 300, 8, 2, [300, 7]), (1, 17, 129, 3, 3, None), (3, 77, 333, 6, 2, [333, 0, 128]),
     (2, 130, 257, 5, 1, [257, 200]), (1, 300, 64, 4, 4, [64]), (2, 64, 1000, 8, 1, [1000, 1]), (1, 257, 513, 14, 2, [500]), (2, 100, 140, 64, 1, [139, 3]),
     (1, 50, 90, 33, 1, None), (1, 700, 300, 2, 2, [129]), (4, 9, 65, 16, 4, [0, 64, 65, 63]),
+    # few CTAs and long loops: cut into parts, some of them without a tile of the shorter entries
+    (1, 40, 3000, 4, 1, [2900]), (3, 20, 2600, 8, 2, [2600, 100, 0]), (1, 2000, 100, 4, 2, None), (2, 1500, 1030, 3, 1, [1030, 600]), (1, 33, 2049, 1, 1, None),
 ]
 
 
@@ -62,7 +64,8 @@ def test_forward_and_gradients(gpu, b, tq, tk, hq, hkv, lengths):
     check(x, lengths, run(x, lengths))
 
 
-@pytest.mark.parametrize("b,tq,tk,hq,hkv,lengths", [(2, 1, 300, 8, 2, [290, 7]), (3, 77, 333, 6, 2, [300, 0, 128]), (2, 200, 1000, 8, 1, [999, 1])])
+@pytest.mark.parametrize("b,tq,tk,hq,hkv,lengths", [(2, 1, 300, 8, 2, [290, 7]), (3, 77, 333, 6, 2, [300, 0, 128]), (2, 200, 1000, 8, 1, [999, 1]),
+                                                      (2, 20, 2600, 8, 2, [2500, 130])])
 def test_padding_is_never_used(gpu, b, tq, tk, hq, hkv, lengths):
     """NaN or infinities behind the lengths: the same bits as zeros there."""
     query, key, value, dout = inputs(gpu, b, tq, tk, hq, hkv)
