@@ -13,8 +13,8 @@
 //   2. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
 //      key (two, half the rows each), P^T and dS^T back into tensor memory as bf16 A operands, dV += P^T dO, dK += dS^T Q.  Tensor memory: dV 128, dK
 //      128, two pairs of 64-column scores, so the scores of the next tile are computed while the softmax works on this one.
-//   3. cross_reduce_kernel, where a grid of whole loops would leave SMs idle: the loops of the first two are cut into parts, whose fp32
-//      sums it adds in order.
+// Where a grid of whole loops would leave SMs idle the loops are cut into parts for the CTAs of a cluster, which add their fp32 sums in order through
+// distributed shared memory (loop_parts.cuh).
 // S and dP are computed twice (1792 instead of 1280 FLOP per pair).  The alternative of the causal backward, dS stored once and streamed
 // back, moves 4 bytes per pair through HBM, 0.62 ps at the measured copy rate, against 0.31 ps for the 512 FLOP at the measured tensor rate.
 //
@@ -53,8 +53,9 @@ constexpr int MMA_WARP = 8;
 constexpr int LOAD_WARP = 9;
 constexpr int TMEM_COLUMNS = 512;
 constexpr float LOG2E = 1.4426950408889634F;
-constexpr int MIN_QUERY_PART = 4;           // key tiles of a part of the query kernel's loop
-constexpr int MIN_KEY_PART = 8;             // row tiles of a part of the key kernel's loop
+constexpr double QUERY_TILE_US = 1.15;      // a key tile of the query kernel's loop
+constexpr double KEY_TILE_US = 0.75;        // a row tile of the key kernel's loop
+constexpr int MOST_KEY_PARTS = 16;          // few keys under many rows: the backward of 64 keys under 4096 x 3 rows 45 us with 8 parts, 38 with 16
 
 __device__ int cross_backward_status = 0;
 
@@ -67,11 +68,9 @@ struct CrossBackwardParams {
     float2* rows;                       // [B, Hkv, Tq, group]: lse * log2(e), delta
     const float* lse;                   // [B, Hq, Tq]
     const int* lengths;                 // null: Tk
-    float* dq_parts;                    // [query_parts][B, Tq, Hq, 128], where there are several
-    float* dk_parts;                    // [key_parts][B, Tk, Hkv, 128]
-    float* dv_parts;
-    int query_parts, key_parts;
-    int batch, tokens, keys, kv_heads, group;
+    __nv_bfloat16 *dq_out, *dk_out, *dv_out;
+    int query_parts, key_parts;         // CTAs (a cluster) that share a loop
+    int tokens, keys, kv_heads, group;
     int sub_tokens, big_tokens;         // tokens of a query tile of each kind
     float scale, scale_log2;
 };
@@ -117,25 +116,22 @@ struct Barriers {
     uint64_t staged[2];             // dV, dK rows are in shared memory
     uint32_t tmem_base;
     int abort_flag;
+    int gave_up;
     alignas(16) float lse2[STAGES][SUB];
     alignas(16) float delta[STAGES][SUB];
 };
 static_assert(sizeof(Barriers) <= MISC_BYTES, "barrier block too large");
+static_assert(2 * RESULT_BYTES <= STAGES * STAGE_BYTES, "the parts' sums take the streamed tiles' place");
 static_assert(offsetof(Barriers, lse2) % 16 == 0 && offsetof(Barriers, delta) % 16 == 0, "16-byte loads of the per-row constants");
 }  // namespace keyside
 
 __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_constant__ CrossBackwardParams p) {
     using namespace keyside;
     extern __shared__ uint8_t smem_raw[];
-    if (*reinterpret_cast<volatile int*>(&cross_backward_status) != 0) {
-        grid_dependency_wait();
-        return;
-    }
     const int entry = blockIdx.z;
     const int kv_head = blockIdx.y;
-    const int key_tiles = (p.keys + BIG - 1) / BIG;
-    const int part = blockIdx.x / key_tiles;
-    const int key_start = (blockIdx.x - part * key_tiles) * BIG;
+    const int part = blockIdx.x % p.key_parts;          // also the rank in the cluster
+    const int key_start = blockIdx.x / p.key_parts * BIG;
     const int rows_per_tile = p.sub_tokens * p.group;
 
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023U) & ~1023U;
@@ -163,6 +159,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
         }
         mbar_init(smem_u32(&bars->final_full), 1);
         bars->abort_flag = 0;
+        // after an earlier launch ran into a time limit nothing is done; the CTAs of a cluster stay to the end all the same
+        bars->gave_up = *reinterpret_cast<volatile int*>(&cross_backward_status);
         mbar_init_fence();
     }
     if (warp == MMA_WARP) {
@@ -185,7 +183,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
     // keys behind the length have gradients of zero: no tiles for them
     const int all_tiles = (p.tokens + p.sub_tokens - 1) / p.sub_tokens;
     const int first_tile = part_begin(all_tiles, part, p.key_parts);
-    const int tile_count = key_start < length ? part_begin(all_tiles, part + 1, p.key_parts) - first_tile : 0;
+    const bool dead = *reinterpret_cast<volatile int*>(&bars->gave_up) != 0;
+    const int tile_count = key_start < length && !dead ? part_begin(all_tiles, part + 1, p.key_parts) - first_tile : 0;
 
     if (warp == LOAD_WARP) {
         if (tile_count > 0 && lane == 0) {
@@ -365,23 +364,19 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
         if (alive && tile_count > 0) {
             alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->final_full), 0, abort_flag, &cross_backward_status));
         }
-        if (alive) {
+        if (alive && !dead) {
             // group 0 stores dV through V's place, group 1 dK through K's
             tc_fence_after_sync();
             const bool keep = key_start + r < length;
             uint8_t* stage = smem + (group == 0 ? 2 * BIG_CHUNK : 0);
             if (p.key_parts > 1) {
-                // keys behind the length are the reduce kernel's zeros
-                float* parts = (group == 0 ? p.dv_parts : p.dk_parts) + static_cast<size_t>(part) * p.batch * p.keys * p.kv_heads * HEAD;
-                const int key0 = key_start + (warp % 4) * 32;
+                // into the streamed tiles' place, dV in front of dK
 #pragma unroll
                 for (int c = 0; c < HEAD / 32 && tile_count > 0; ++c) {
                     uint32_t values[32];
                     tmem_ld_x32(tmem_base + lane_base + (group == 0 ? TMEM_DV : TMEM_DK) + c * 32, values);
                     tmem_wait_ld();
-                    store_f32_rows(stage + (warp % 4) * 4096, lane, values, [&](int row) -> float* {
-                        return key0 + row < length ? parts + ((static_cast<size_t>(entry) * p.keys + key0 + row) * p.kv_heads + kv_head) * HEAD + c * 32 : nullptr;
-                    });
+                    result_store32(smem + RESIDENT_BYTES + group * RESULT_BYTES, r, c * 32, values);
                 }
             } else {
 #pragma unroll
@@ -404,6 +399,31 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
                 }
             }
         }
+    }
+
+    if (p.key_parts > 1) {
+        // each CTA its share of the 2 x 128 rows of dV and dK
+        __syncwarp();
+        cluster_sync_all();
+        constexpr int WARPS = THREADS / 32;
+        const int row_end = dead ? 0 : part_begin(2 * BIG, part + 1, p.key_parts);
+        for (int first = part_begin(2 * BIG, part, p.key_parts) + warp; first < row_end; first += SUM_ROWS * WARPS) {
+            float4 sums[SUM_ROWS];
+            // (dK lies behind dV, so that row 128 + k of the two together is row k of dK)
+            cluster_sums(sums, stage_smem, lane, 0, key_start < length ? p.key_parts : 0, first, WARPS, row_end, [](int, int) { return 1.0F; });
+#pragma unroll
+            for (int k = 0; k < SUM_ROWS; ++k) {
+                const int row = first + k * WARPS;
+                const int key = key_start + row % BIG;
+                if (row < row_end && key < p.keys) {
+                    const uint2 packed = make_uint2(pack_bf16x2(sums[k].x, sums[k].y), pack_bf16x2(sums[k].z, sums[k].w));
+                    reinterpret_cast<uint2*>((row < BIG ? p.dv_out : p.dk_out) + ((static_cast<size_t>(entry) * p.keys + key) * p.kv_heads + kv_head) * HEAD)[lane] =
+                        key < length ? packed : make_uint2(0, 0);
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();             // nobody leaves while others read
     }
 
     __syncwarp();
@@ -454,23 +474,20 @@ struct Barriers {
     uint64_t delta_full;
     uint32_t tmem_base;
     int abort_flag;
+    int gave_up;
     float delta[2][2][BIG];     // each half's share of sum_d dO O, and with one key tile of sum_k P dP
 };
 static_assert(sizeof(Barriers) <= MISC_BYTES, "barrier block too large");
+static_assert(RESULT_BYTES <= K_SLOTS * TILE_BYTES, "the part's sums take K's place");
 }  // namespace queryside
 
 __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_constant__ CrossBackwardParams p) {
     using namespace queryside;
     extern __shared__ uint8_t smem_raw[];
-    if (*reinterpret_cast<volatile int*>(&cross_backward_status) != 0) {
-        grid_dependency_wait();
-        return;
-    }
     const int entry = blockIdx.z;
     const int kv_head = blockIdx.y;
-    const int row_tiles = (p.tokens + p.big_tokens - 1) / p.big_tokens;
-    const int part = blockIdx.x / row_tiles;
-    const int token0 = (blockIdx.x - part * row_tiles) * p.big_tokens;
+    const int part = blockIdx.x % p.query_parts;        // also the rank in the cluster
+    const int token0 = blockIdx.x / p.query_parts * p.big_tokens;
     const int rows_per_tile = p.big_tokens * p.group;
 
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023U) & ~1023U;
@@ -503,6 +520,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
         mbar_init(smem_u32(&bars->staged), SOFTMAX_THREADS);
         mbar_init(smem_u32(&bars->delta_full), SOFTMAX_THREADS);
         bars->abort_flag = 0;
+        // after an earlier launch ran into a time limit nothing is done; the CTAs of a cluster stay to the end all the same
+        bars->gave_up = *reinterpret_cast<volatile int*>(&cross_backward_status);
         mbar_init_fence();
     }
     if (warp == MMA_WARP) {
@@ -517,7 +536,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
     const int length = length_of(p, entry);
     const int all_tiles = (length + KEYS - 1) / KEYS;
     const int first_tile = part_begin(all_tiles, part, p.query_parts);
-    const int tile_count = part_begin(all_tiles, part + 1, p.query_parts) - first_tile;
+    const bool dead = *reinterpret_cast<volatile int*>(&bars->gave_up) != 0;
+    const int tile_count = dead ? 0 : part_begin(all_tiles, part + 1, p.query_parts) - first_tile;
     const int left = length - first_tile * KEYS;        // keys from the first tile on
 
     if (warp == LOAD_WARP) {
@@ -728,7 +748,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
             }
         }
         // (the last part always has a tile of an entry that has any)
-        float2* row = valid && half == 0 && part + 1 == p.query_parts && length > 0
+        float2* row = valid && half == 0 && part + 1 == p.query_parts && tile_count > 0
                           ? p.rows + ((static_cast<size_t>(entry) * p.kv_heads + kv_head) * p.tokens + token) * p.group + r % p.group
                           : nullptr;
         if (row != nullptr && alive) {
@@ -798,22 +818,15 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
         if (alive && tile_count > 0) {
             alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->final_full), 0, abort_flag, &cross_backward_status));
         }
-        if (alive) {
+        if (alive && !dead) {
             tc_fence_after_sync();
             if (p.query_parts > 1) {
-                float* parts = p.dq_parts + static_cast<size_t>(part) * p.batch * p.tokens * p.kv_heads * p.group * HEAD;
 #pragma unroll
                 for (int c = 0; c < 2 && tile_count > 0; ++c) {
                     uint32_t values[32];
                     tmem_ld_x32(tmem_base + lane_base + TMEM_DQ + half * 64 + c * 32, values);
                     tmem_wait_ld();
-                    store_f32_rows(smem + warp * 4096, lane, values, [&](int index) -> float* {
-                        const int at = (warp % 4) * 32 + index;
-                        const int t = token0 + at / p.group;
-                        return at < rows_per_tile && t < p.tokens
-                                   ? parts + ((static_cast<size_t>(entry) * p.tokens + t) * p.kv_heads * p.group + kv_head * p.group + at % p.group) * HEAD + half * 64 + c * 32
-                                   : nullptr;
-                    });
+                    result_store32(smem + Q_BYTES, r, half * 64 + c * 32, values);     // into K's place
                 }
             } else {
 #pragma unroll
@@ -838,6 +851,30 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
         }
     }
 
+    if (p.query_parts > 1) {
+        // each CTA its share of the rows; parts without tiles have left nothing
+        __syncwarp();
+        cluster_sync_all();
+        constexpr int WARPS = THREADS / 32;
+        const int rows = min(p.big_tokens, p.tokens - token0) * p.group;
+        const int row_end = dead ? 0 : part_begin(rows, part + 1, p.query_parts);
+        for (int first = part_begin(rows, part, p.query_parts) + warp; first < row_end; first += SUM_ROWS * WARPS) {
+            float4 sums[SUM_ROWS];
+            cluster_sums(sums, k_ring, lane, parts_without(all_tiles, p.query_parts), p.query_parts, first, WARPS, row_end, [](int, int) { return 1.0F; });
+#pragma unroll
+            for (int k = 0; k < SUM_ROWS; ++k) {
+                const int row = first + k * WARPS;
+                if (row < row_end) {
+                    reinterpret_cast<uint2*>(p.dq_out + ((static_cast<size_t>(entry) * p.tokens + token0 + row / p.group) * p.kv_heads * p.group + kv_head * p.group +
+                                                         row % p.group) * HEAD)[lane] =
+                        make_uint2(pack_bf16x2(sums[k].x, sums[k].y), pack_bf16x2(sums[k].z, sums[k].w));
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();             // nobody leaves while others read
+    }
+
     __syncwarp();
     tc_fence_before_sync();
     __syncthreads();
@@ -852,62 +889,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
     }
 }
 
-// ---------------------------------------------------------------------------
-// Parts added in order; a thread takes four columns of a row
-// ---------------------------------------------------------------------------
-__device__ __forceinline__ uint2 sum_parts(const float* parts, size_t offset, size_t stride, int first, int last) {
-    float4 sum = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-#pragma unroll 4
-    for (int part = first; part < last; ++part) {
-        const float4 x = *reinterpret_cast<const float4*>(parts + part * stride + offset);
-        sum.x += x.x;
-        sum.y += x.y;
-        sum.z += x.z;
-        sum.w += x.w;
-    }
-    return make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
-}
-
-__global__ void __launch_bounds__(256) cross_reduce_kernel(const __grid_constant__ CrossBackwardParams p, uint2* dq, uint2* dk, uint2* dv) {
-    const size_t entry_query = static_cast<size_t>(p.tokens) * p.kv_heads * p.group * (HEAD / 4);       // units of an entry
-    const size_t entry_key = static_cast<size_t>(p.keys) * p.kv_heads * (HEAD / 4);
-    const size_t queries = p.query_parts > 1 ? p.batch * entry_query : 0;
-    const size_t keys = p.key_parts > 1 ? p.batch * entry_key : 0;
-    const size_t step = static_cast<size_t>(gridDim.x) * 256;
-    grid_dependency_wait();
-    for (size_t i = static_cast<size_t>(blockIdx.x) * 256 + threadIdx.x; i < queries + keys; i += step) {
-        if (i < queries) {
-            // a part without tiles has written nothing
-            const int tiles = (length_of(p, static_cast<int>(i / entry_query)) + queryside::KEYS - 1) / queryside::KEYS;
-            uint2 result = make_uint2(0, 0);
-            if (tiles >= p.query_parts) {
-                result = sum_parts(p.dq_parts, i * 4, p.batch * entry_query * 4, 0, p.query_parts);
-            } else {
-                float4 sum = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-                for (int part = 0; part < p.query_parts; ++part) {
-                    if (part_begin(tiles, part, p.query_parts) < part_begin(tiles, part + 1, p.query_parts)) {
-                        const float4 x = *reinterpret_cast<const float4*>(p.dq_parts + part * (p.batch * entry_query * 4) + i * 4);
-                        sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
-                    }
-                }
-                result = make_uint2(pack_bf16x2(sum.x, sum.y), pack_bf16x2(sum.z, sum.w));
-            }
-            dq[i] = result;
-        } else {
-            const size_t at = i - queries;
-            const int entry = static_cast<int>(at / entry_key);
-            const int key = static_cast<int>((at - entry * entry_key) / (p.kv_heads * (HEAD / 4)));
-            const bool present = key < length_of(p, entry);
-            dk[at] = present ? sum_parts(p.dk_parts, at * 4, keys * 4, 0, p.key_parts) : make_uint2(0, 0);
-            dv[at] = present ? sum_parts(p.dv_parts, at * 4, keys * 4, 0, p.key_parts) : make_uint2(0, 0);
-        }
-    }
-}
-
 struct Plan {
     int query_parts, key_parts;
-    std::size_t rows_bytes, query_bytes, key_bytes;         // of the row constants, of all parts of dQ, of all parts of dK (and dV)
-    std::size_t bytes() const { return rows_bytes + query_bytes + 2 * key_bytes; }
 };
 
 Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
@@ -916,14 +899,7 @@ Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
     const long long row_tiles = (queries + BIG / group - 1LL) / (BIG / group);
     const long long sub_tiles = (queries + SUB / group - 1LL) / (SUB / group);
     const long long pairs = static_cast<long long>(batch) * kv_heads;
-    Plan plan{};
-    plan.query_parts = loop_parts(row_tiles * pairs, key_tiles, MIN_QUERY_PART);
-    plan.key_parts = loop_parts(key_tiles * pairs, sub_tiles, MIN_KEY_PART);
-    const std::size_t query_rows = static_cast<std::size_t>(batch) * queries * heads, key_rows = static_cast<std::size_t>(batch) * keys * kv_heads;
-    plan.rows_bytes = (query_rows * sizeof(float2) + 15) / 16 * 16;
-    plan.query_bytes = plan.query_parts > 1 ? plan.query_parts * query_rows * HEAD * sizeof(float) : 0;
-    plan.key_bytes = plan.key_parts > 1 ? plan.key_parts * key_rows * HEAD * sizeof(float) : 0;
-    return plan;
+    return {loop_parts(row_tiles * pairs, key_tiles, QUERY_TILE_US, 8), loop_parts(key_tiles * pairs, sub_tiles, KEY_TILE_US, MOST_KEY_PARTS)};
 }
 
 void configure() {
@@ -934,6 +910,7 @@ void configure() {
         return;
     }
     CUDA_CHECK(cudaFuncSetAttribute(cross_key_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, keyside::SMEM_BYTES));
+    CUDA_CHECK(cudaFuncSetAttribute(cross_key_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     CUDA_CHECK(cudaFuncSetAttribute(cross_query_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, queryside::SMEM_BYTES));
     if (device < 16) {
         done[device] = true;
@@ -961,10 +938,7 @@ std::size_t flash_cross_backward_workspace_bytes(int batch_size, int query_lengt
     if (batch_size <= 0 || query_length <= 0 || key_length <= 0 || query_heads <= 0 || key_value_heads <= 0) {
         return 0;
     }
-    if (query_heads % key_value_heads != 0 || query_heads / key_value_heads > SUB) {
-        return 0;                   // refused by the call
-    }
-    return make_plan(batch_size, query_length, key_length, query_heads, key_value_heads).bytes();
+    return static_cast<std::size_t>(batch_size) * query_length * query_heads * sizeof(float2);
 }
 
 void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key_gradient, __nv_bfloat16* value_gradient,
@@ -996,32 +970,24 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     p.dk = make_bf16_batched_tile_map(key_gradient, batch_size, key_length, wide, BIG);
     p.dv = make_bf16_batched_tile_map(value_gradient, batch_size, key_length, wide, BIG);
     const Plan plan = make_plan(batch_size, query_length, key_length, query_heads, key_value_heads);
-    uint8_t* memory = static_cast<uint8_t*>(workspace);
-    p.rows = reinterpret_cast<float2*>(memory);
-    p.dq_parts = reinterpret_cast<float*>(memory + plan.rows_bytes);
-    p.dk_parts = reinterpret_cast<float*>(memory + plan.rows_bytes + plan.query_bytes);
-    p.dv_parts = reinterpret_cast<float*>(memory + plan.rows_bytes + plan.query_bytes + plan.key_bytes);
+    p.rows = static_cast<float2*>(workspace);
+    p.dq_out = query_gradient;
+    p.dk_out = key_gradient;
+    p.dv_out = value_gradient;
     p.query_parts = plan.query_parts;
     p.key_parts = plan.key_parts;
     p.lse = logsumexp;
     p.lengths = key_lengths;
-    p.batch = batch_size;
     p.tokens = query_length;
     p.keys = key_length;
     p.kv_heads = key_value_heads;
     p.scale = scale;
     p.scale_log2 = scale * LOG2E;
     configure();
-    launch_chained(cross_query_kernel, dim3((query_length + p.big_tokens - 1) / p.big_tokens * plan.query_parts, key_value_heads, batch_size), dim3(THREADS),
-                   queryside::SMEM_BYTES, stream, p);
-    launch_chained(cross_key_kernel, dim3((key_length + BIG - 1) / BIG * plan.key_parts, key_value_heads, batch_size), dim3(THREADS), keyside::SMEM_BYTES,
-                   stream, p);
-    if (plan.query_parts > 1 || plan.key_parts > 1) {
-        const long long units = ((plan.query_parts > 1 ? static_cast<long long>(batch_size) * query_length * query_heads : 0) +
-                                 (plan.key_parts > 1 ? static_cast<long long>(batch_size) * key_length * key_value_heads : 0)) * (HEAD / 4);
-        launch_chained(cross_reduce_kernel, dim3(static_cast<unsigned>(std::min((units + 255) / 256, SMS * 8))), dim3(256), 0, stream, p,
-                       reinterpret_cast<uint2*>(query_gradient), reinterpret_cast<uint2*>(key_gradient), reinterpret_cast<uint2*>(value_gradient));
-    }
+    launch_chained_clusters(cross_query_kernel, dim3((query_length + p.big_tokens - 1) / p.big_tokens * plan.query_parts, key_value_heads, batch_size),
+                            plan.query_parts, dim3(THREADS), queryside::SMEM_BYTES, stream, p);
+    launch_chained_clusters(cross_key_kernel, dim3((key_length + BIG - 1) / BIG * plan.key_parts, key_value_heads, batch_size), plan.key_parts, dim3(THREADS),
+                            keyside::SMEM_BYTES, stream, p);
 }
 
 }  // namespace dscuda

@@ -11,8 +11,8 @@
 // entry's length (a weight of zero does not keep their NaN out of P V) and complete the third warpgroup, which hands registers to the
 // softmax.  The schedule is that of prefill_forward.cu, where its measurements stand.
 //
-// Small problems: where pairs of tiles would leave SMs idle a CTA takes one tile, and where that is not enough the loop over the keys is cut into parts,
-// whose fp32 results cross_combine_kernel joins.
+// Small problems: where pairs of tiles would leave SMs idle a CTA takes one tile, and where that is not enough the loop over the keys is cut into parts
+// for the CTAs of a cluster, which join their fp32 sums through distributed shared memory (loop_parts.cuh).
 //
 // Few rows to a key head (single tokens) go to flash_decode.cu instead, which splits the keys over the SMs.
 //
@@ -38,7 +38,7 @@ constexpr int CHUNK = 128 * 128;            // 16 KB: 128 rows x 64 bf16, or 64 
 constexpr int RING = 10;
 constexpr int PER_TILE = 4;                 // ring chunks of a key tile: two of K, two of V
 constexpr int Q_BYTES = 4 * CHUNK;
-constexpr int MISC_BYTES = 1024;
+constexpr int MISC_BYTES = 2048;
 constexpr int SMEM_BYTES = Q_BYTES + RING * CHUNK + MISC_BYTES + 1024;
 constexpr int THREADS = 384;
 constexpr int MMA_WARP = 8;
@@ -47,6 +47,7 @@ constexpr int TAIL_WARP = 10;
 constexpr int TMEM_COLUMNS = 512;           // S0 | S1 | O0 | O1
 constexpr float RESCALE_THRESHOLD = 8.0F;   // log2 units; below it the old row maximum is kept
 constexpr float LOG2E = 1.4426950408889634F;
+constexpr float LN2 = 0.6931471805599453F;
 
 __device__ int cross_forward_status = 0;
 
@@ -57,12 +58,11 @@ struct CrossForwardParams {
     CUtensorMap out;            // like q
     float* lse;                 // [B, Hq, Tq]
     const int* lengths;         // null: Tk
-    float* part_out;            // [parts][B, Tq, Hq, 128], where there are several
-    float* part_lse;            // [parts][B, Hq, Tq], log2 domain
-    int batch, tokens, keys, heads, group;
+    __nv_bfloat16* output;      // [B, Tq, Hq, 128]
+    int tokens, keys, heads, group;
     int tile_tokens;            // tokens of a query tile
     int cta_tiles;              // query tiles of a CTA: 1 or 2
-    int parts;                  // CTAs that share the keys of a query tile
+    int parts;                  // CTAs (a cluster) that share the keys of a query tile; then cta_tiles is 1
     float scale, scale_log2;
 };
 
@@ -77,21 +77,18 @@ struct Barriers {
     uint64_t tail_full[2];
     uint32_t tmem_base;
     int abort_flag;
+    int gave_up;
+    float2 row_sums[TILE];      // parts: reference (log2 domain) and sum of each row
 };
 static_assert(sizeof(Barriers) <= MISC_BYTES, "barrier block too large");
 
 __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_constant__ CrossForwardParams p) {
     extern __shared__ uint8_t smem_raw[];
-    if (*reinterpret_cast<volatile int*>(&cross_forward_status) != 0) {
-        grid_dependency_wait();
-        return;
-    }
     const int entry = blockIdx.z;
     const int kv_head = blockIdx.y;
     const int row_tiles = (p.tokens + p.tile_tokens - 1) / p.tile_tokens;
-    const int row_ctas = (row_tiles + p.cta_tiles - 1) / p.cta_tiles;
-    const int part = blockIdx.x / row_ctas;
-    const int tile0 = (blockIdx.x - part * row_ctas) * p.cta_tiles;
+    const int part = blockIdx.x % p.parts;              // also the rank in the cluster
+    const int tile0 = blockIdx.x / p.parts * p.cta_tiles;
     const bool second = p.cta_tiles == 2 && tile0 + 1 < row_tiles;
 
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023U) & ~1023U;
@@ -116,6 +113,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
             mbar_init(smem_u32(&bars->ring_empty[i]), 1);
         }
         bars->abort_flag = 0;
+        // after an earlier launch ran into a time limit nothing is done; the CTAs of a cluster stay to the end all the same
+        bars->gave_up = *reinterpret_cast<volatile int*>(&cross_forward_status);
         mbar_init_fence();
     }
     if (warp == MMA_WARP) {
@@ -135,7 +134,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
     const int length = p.lengths == nullptr ? p.keys : min(max(p.lengths[entry], 0), p.keys);
     const int all_tiles = (length + TILE - 1) / TILE;
     const int first_tile = part_begin(all_tiles, part, p.parts);
-    const int tile_count = part_begin(all_tiles, part + 1, p.parts) - first_tile;
+    const bool dead = *reinterpret_cast<volatile int*>(&bars->gave_up) != 0;
+    const int tile_count = dead ? 0 : part_begin(all_tiles, part + 1, p.parts) - first_tile;
     const int left = length - first_tile * TILE;        // keys from the first tile on
     // what lies between the length and the end of the entry's states may be anything; behind that end the loads give zeros
     const int tail_keys = length < p.keys ? min(left - (tile_count - 1) * TILE, TILE) : TILE;
@@ -386,37 +386,21 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
             tc_fence_before_sync();
             mbar_arrive(smem_u32(&bars->p_full[i]));
         }
-        const bool active = i == 0 || second;
+        const bool active = !dead && (i == 0 || second);
         if (alive && count > 0) {
             alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->s_full[i]), count & 1, abort_flag, &cross_forward_status));
         }
         if (alive && active && p.parts > 1) {
-            // (a part without tiles has nothing to write)
-            if (count > 0) {
-                tc_fence_after_sync();
-                const float inverse = 1.0F / l_sum;
-                const size_t rows = static_cast<size_t>(p.batch) * p.tokens * p.heads;
+            // the part's sums into the ring, which is idle by now
+            tc_fence_after_sync();
 #pragma unroll
-                for (int c = 0; c < HEAD / 32; ++c) {
-                    uint32_t o[32];
-                    tmem_ld_x32(o_tmem + c * 32, o);
-                    tmem_wait_ld();
-#pragma unroll
-                    for (int e = 0; e < 32; ++e) {
-                        o[e] = __float_as_uint(__uint_as_float(o[e]) * inverse);
-                    }
-                    store_f32_rows(smem + 2 * i * CHUNK + (warp % 4) * 4096, lane, o, [&](int index) -> float* {
-                        const int at = (warp % 4) * 32 + index;
-                        const int t = (tile0 + i) * p.tile_tokens + at / p.group;
-                        return at < p.tile_tokens * p.group && t < p.tokens
-                                   ? p.part_out + (part * rows + (static_cast<size_t>(entry) * p.tokens + t) * p.heads + kv_head * p.group + at % p.group) * HEAD + c * 32
-                                   : nullptr;
-                    });
-                }
-                if (valid) {
-                    p.part_lse[part * rows + (lse - p.lse)] = m_ref * p.scale_log2 + log2f(l_sum);
-                }
+            for (int c = 0; c < HEAD / 32 && count > 0; ++c) {
+                uint32_t o[32];
+                tmem_ld_x32(o_tmem + c * 32, o);
+                tmem_wait_ld();
+                result_store32(smem + Q_BYTES, r, c * 32, o);
             }
+            bars->row_sums[r] = count > 0 ? make_float2(m_ref * p.scale_log2, l_sum) : make_float2(-INFINITY, 0.0F);
         } else if (alive && active) {
             // rows of 64 columns into the tile's Q chunks (idle by now), from where a TMA store takes them
             tc_fence_after_sync();
@@ -459,6 +443,54 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
         }
     }
 
+    // ---- parts: each CTA its share of the rows ----
+    if (p.parts > 1) {
+        __syncwarp();
+        cluster_sync_all();
+        const int rows = min(p.tile_tokens, p.tokens - tile0 * p.tile_tokens) * p.group;
+        const int row_end = dead ? 0 : part_begin(rows, part + 1, p.parts);
+        constexpr int WARPS = THREADS / 32;
+        for (int first = part_begin(rows, part, p.parts) + warp; first < row_end; first += SUM_ROWS * WARPS) {
+            // lane 8 k + n: reference and sum of part n (of at most 8) for the warp's k-th row
+            float2 sums = make_float2(-INFINITY, 0.0F);
+            const int mine = first + lane / 8 * WARPS;
+            if (lane % 8 < p.parts && lane / 8 < SUM_ROWS && mine < row_end) {
+                sums = cluster_load2(map_to_cta(smem_u32(&bars->row_sums[mine]), lane % 8));
+            }
+            float top = sums.x;
+#pragma unroll
+            for (int offset = 4; offset > 0; offset >>= 1) {
+                top = fmaxf(top, __shfl_xor_sync(0xffffffffU, top, offset));
+            }
+            const float reference = top == -INFINITY ? 0.0F : top;
+            float weight = exp2_approx(sums.x - reference);
+            float total = weight * sums.y;
+#pragma unroll
+            for (int offset = 4; offset > 0; offset >>= 1) {
+                total += __shfl_xor_sync(0xffffffffU, total, offset);
+            }
+            weight = total == 0.0F ? 0.0F : weight / total;
+            float4 value[SUM_ROWS];
+            cluster_sums(value, ring_smem, lane, parts_without(all_tiles, p.parts), p.parts, first, WARPS, row_end,
+                         [&](int k, int other) { return __shfl_sync(0xffffffffU, weight, 8 * k + other); });
+#pragma unroll
+            for (int k = 0; k < SUM_ROWS; ++k) {
+                const int row = first + k * WARPS;
+                if (row < row_end) {
+                    const int token = tile0 * p.tile_tokens + row / p.group;
+                    const int head = kv_head * p.group + row % p.group;
+                    reinterpret_cast<uint2*>(p.output + ((static_cast<size_t>(entry) * p.tokens + token) * p.heads + head) * HEAD)[lane] =
+                        make_uint2(pack_bf16x2(value[k].x, value[k].y), pack_bf16x2(value[k].z, value[k].w));
+                    if (lane == 8 * k) {
+                        p.lse[(static_cast<size_t>(entry) * p.heads + head) * p.tokens + token] = total == 0.0F ? -INFINITY : reference * LN2 + logf(total);
+                    }
+                }
+            }
+        }
+        __syncwarp();
+        cluster_sync_all();             // nobody leaves while others read
+    }
+
     // ---- teardown: every path reaches this point ----
     __syncwarp();
     tc_fence_before_sync();
@@ -474,51 +506,11 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
     }
 }
 
-// Joins the parts of every row in the order of their keys; a warp to a row, four columns to a lane.
-__global__ void __launch_bounds__(128) cross_combine_kernel(const __grid_constant__ CrossForwardParams p, uint2* out) {
-    const long long rows = static_cast<long long>(p.batch) * p.tokens * p.heads;
-    const long long row = blockIdx.x * 4LL + threadIdx.x / 32;          // (entry, token, head)
-    const int lane = threadIdx.x % 32;
-    if (row >= rows) {
-        return;
-    }
-    const int head = static_cast<int>(row % p.heads);
-    const long long at = row / p.heads;
-    const int entry = static_cast<int>(at / p.tokens);
-    const long long lse_index = (static_cast<long long>(entry) * p.heads + head) * p.tokens + at % p.tokens;
-    grid_dependency_wait();
-    const int length = p.lengths == nullptr ? p.keys : min(max(p.lengths[entry], 0), p.keys);
-    const int tiles = (length + TILE - 1) / TILE;
-    auto present = [&](int part) { return part_begin(tiles, part, p.parts) < part_begin(tiles, part + 1, p.parts); };
-    float top = -INFINITY;
-    for (int part = 0; part < p.parts; ++part) {
-        top = present(part) ? fmaxf(top, p.part_lse[part * rows + lse_index]) : top;
-    }
-    const float reference = top == -INFINITY ? 0.0F : top;
-    float sum = 0.0F;
-    float4 value = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-    for (int part = 0; part < p.parts; ++part) {
-        if (present(part)) {
-            const float weight = exp2_approx(p.part_lse[part * rows + lse_index] - reference);
-            const float4 x = *reinterpret_cast<const float4*>(p.part_out + (part * rows + row) * HEAD + lane * 4);
-            sum += weight;
-            value = make_float4(value.x + weight * x.x, value.y + weight * x.y, value.z + weight * x.z, value.w + weight * x.w);
-        }
-    }
-    const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
-    out[row * 32 + lane] = make_uint2(pack_bf16x2(value.x * inverse, value.y * inverse), pack_bf16x2(value.z * inverse, value.w * inverse));
-    if (lane == 0) {
-        p.lse[lse_index] = sum == 0.0F ? -INFINITY : (reference + log2f(sum)) * 0.6931471805599453F;
-    }
-}
-
 // How a call's rows and keys are dealt to CTAs.
-constexpr int MIN_PART = 4;                 // key tiles of a part
+constexpr double TILE_US = 1.75;            // a key tile in a CTA with one query tile
 
 struct Plan {
     int cta_tiles, row_ctas, parts;
-    std::size_t rows;
-    std::size_t bytes() const { return parts > 1 ? parts * rows * (HEAD + 1) * sizeof(float) : 0; }
 };
 
 Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
@@ -528,8 +520,8 @@ Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
     Plan plan{};
     plan.cta_tiles = row_tiles * pairs <= SMS ? 1 : 2;
     plan.row_ctas = static_cast<int>((row_tiles + plan.cta_tiles - 1) / plan.cta_tiles);
-    plan.parts = loop_parts(plan.row_ctas * pairs, (keys + TILE - 1LL) / TILE, MIN_PART);
-    plan.rows = static_cast<std::size_t>(batch) * queries * heads;
+    // (with two tiles to a CTA there is one for every second SM already)
+    plan.parts = plan.cta_tiles == 1 ? loop_parts(plan.row_ctas * pairs, (keys + TILE - 1LL) / TILE, TILE_US, 8) : 1;
     return plan;
 }
 
@@ -594,13 +586,7 @@ std::size_t flash_cross_forward_workspace_bytes(int batch_size, int query_length
         return 0;
     }
     const long long rows = static_cast<long long>(query_length) * (query_heads / key_value_heads);
-    if (rows <= FEW_ROWS) {
-        return internal::few_rows_workspace_bytes(batch_size, key_value_heads, rows);
-    }
-    if (query_heads % key_value_heads != 0 || query_heads / key_value_heads > 64) {
-        return 0;                   // refused by the call
-    }
-    return make_plan(batch_size, query_length, key_length, query_heads, key_value_heads).bytes();
+    return rows <= FEW_ROWS ? internal::few_rows_workspace_bytes(batch_size, key_value_heads, rows) : 0;
 }
 
 void flash_cross_forward_cuda(__nv_bfloat16* output, float* logsumexp, const __nv_bfloat16* query, const __nv_bfloat16* key,
@@ -640,16 +626,11 @@ void flash_cross_forward_cuda(__nv_bfloat16* output, float* logsumexp, const __n
     p.scale = scale;
     p.scale_log2 = scale * LOG2E;
     const Plan plan = make_plan(batch_size, query_length, key_length, query_heads, key_value_heads);
-    p.batch = batch_size;
+    p.output = output;
     p.cta_tiles = plan.cta_tiles;
     p.parts = plan.parts;
-    p.part_out = static_cast<float*>(workspace);
-    p.part_lse = p.part_out + plan.parts * plan.rows * HEAD;
     configure();
-    launch_chained(cross_forward_kernel, dim3(plan.row_ctas * plan.parts, key_value_heads, batch_size), dim3(THREADS), SMEM_BYTES, stream, p);
-    if (plan.parts > 1) {
-        launch_chained(cross_combine_kernel, dim3(static_cast<unsigned>((plan.rows + 3) / 4)), dim3(128), 0, stream, p, reinterpret_cast<uint2*>(output));
-    }
+    launch_chained_clusters(cross_forward_kernel, dim3(plan.row_ctas * plan.parts, key_value_heads, batch_size), plan.parts, dim3(THREADS), SMEM_BYTES, stream, p);
 }
 
 }  // namespace dscuda

@@ -1,6 +1,9 @@
-// Loops over tiles that are cut into parts, a CTA each, where whole loops would leave SMs idle; the parts' fp32 results are joined in order by
-// another kernel.
+// Loops over tiles that are cut into parts where whole loops would leave SMs idle: the CTAs of a cluster take a part each, keep their fp32
+// results in their own shared memory and read one another's (distributed shared memory) to add them in order.  No scratch in HBM, no
+// second kernel.
 #pragma once
+
+#include "sm100_primitives.cuh"
 
 #include <cuda_runtime.h>
 
@@ -10,37 +13,99 @@
 namespace dscuda {
 
 constexpr long long SMS = 148;
+// Clusters of 1, 2 .. 8 and of 16 CTAs, one CTA to an SM, that a B200 holds at a time (cudaOccupancyMaxActiveClusters: a cluster stays inside one of
+// the groups of 16 to 20 SMs that share a network).  One more waits for a whole wave: 16 clusters of 8 took 42 us where 15 of 7 take 27.
+constexpr int ACTIVE_CLUSTERS[17] = {0, 148, 74, 45, 33, 26, 22, 15, 15, 0, 0, 0, 0, 0, 0, 0, 7};
 
-// Parts that a loop of `tiles` tiles is cut into when `ctas` whole loops would run: enough CTAs for every SM, parts of at least MIN_PART tiles, and no
-// cut that saves less than the reduce kernel costs.
-inline int loop_parts(long long ctas, long long tiles, int min_part) {
-    const long long parts = std::min(SMS / std::max(ctas, 1LL), tiles / min_part);
-    return parts >= 2 ? static_cast<int>(parts) : 1;
-}
+// What a cluster costs beside its loops: launch, two cluster barriers, the reads.  40 heads' rows over 4 key tiles: 11.2 us whole, 11.4 in four parts.
+constexpr double CLUSTER_US = 4.3;
 
-// The share of the loop over `count` tiles that part `part` of `parts` has; the last part's is never empty.
-__device__ __forceinline__ int part_begin(int count, int part, int parts) {
-    return static_cast<int>(static_cast<long long>(count) * part / parts);
-}
-
-// Partial sums: a warp's 32 rows of 32 fp32 columns through 4 KB of shared memory, so that a store instruction writes whole 128-byte lines.
-template <class RowPointer>
-__device__ __forceinline__ void store_f32_rows(uint8_t* slab, int lane, const uint32_t* values, RowPointer row_pointer) {
-#pragma unroll
-    for (int u = 0; u < 8; ++u) {
-        *reinterpret_cast<uint4*>(slab + lane * 128 + ((u ^ (lane & 7)) * 16)) = make_uint4(values[4 * u], values[4 * u + 1], values[4 * u + 2], values[4 * u + 3]);
-    }
-    __syncwarp();
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int row = 4 * i + lane / 8;
-        const uint4 v = *reinterpret_cast<const uint4*>(slab + row * 128 + (((lane % 8) ^ (row & 7)) * 16));
-        float* dst = row_pointer(row);
-        if (dst != nullptr) {
-            reinterpret_cast<uint4*>(dst)[lane % 8] = v;
+// Parts that a loop of `tiles` tiles of `tile_us` microseconds is cut into when `ctas` whole loops would run: the cluster size (up to `most`: 8 is portable, 16 has
+// to be allowed) of the shortest time, of those of which all clusters run at once.
+inline int loop_parts(long long ctas, long long tiles, double tile_us, int most) {
+    int best = 1;
+    double best_us = static_cast<double>(tiles) * tile_us;
+    for (int parts = 2; parts <= most && parts <= tiles; ++parts) {
+        const double us = static_cast<double>((tiles + parts - 1) / parts) * tile_us + CLUSTER_US;
+        if (ctas <= ACTIVE_CLUSTERS[parts] && us < best_us) {
+            best = parts;
+            best_us = us;
         }
     }
-    __syncwarp();
+    return best;
+}
+
+// Where part `part` of `parts` begins in a loop of `count` tiles.  With fewer tiles than parts the last ones take one each and the first
+// parts_without(count, parts) none.
+__device__ __forceinline__ int part_begin(int count, int part, int parts) {
+    return count < parts ? max(0, count - parts + part) : static_cast<int>(static_cast<long long>(count) * part / parts);
+}
+
+__device__ __forceinline__ int parts_without(int count, int parts) {
+    return max(0, parts - count);
+}
+
+// A CTA's result of 128 rows x 128 fp32 columns in shared memory: 512 bytes to a row, 16-byte units swizzled so that neither a thread to a row
+// (writing) nor a warp to a row (reading) meets bank conflicts.
+constexpr int RESULT_BYTES = 128 * 512;
+
+__device__ __forceinline__ uint32_t result_unit(int row, int unit) {
+    return static_cast<uint32_t>(row * 512 + ((unit ^ (row & 7)) * 16));
+}
+
+__device__ __forceinline__ void result_store32(uint8_t* result, int row, int column, const uint32_t* values) {
+#pragma unroll
+    for (int u = 0; u < 8; ++u) {
+        *reinterpret_cast<uint4*>(result + result_unit(row, column / 4 + u)) = make_uint4(values[4 * u], values[4 * u + 1], values[4 * u + 2], values[4 * u + 3]);
+    }
+}
+
+// 16 bytes of another CTA's shared memory (address from sm100::map_to_cta).
+__device__ __forceinline__ float4 cluster_load4(uint32_t addr) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+    return v;
+}
+
+__device__ __forceinline__ float2 cluster_load2(uint32_t addr) {
+    float2 v;
+    asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
+    return v;
+}
+
+// Rows of the results of `parts` CTAs added in order, by a whole warp, a lane to each 16-byte unit: rows first and first + step, as far as they are
+// below `end`, times weight(k, part) for the k-th of them.  Parts below `skipped` have left nothing.  A read from another CTA takes most of a
+// microsecond, so those of two rows and four parts are on the way at once.
+constexpr int SUM_ROWS = 2;
+
+template <class Weight>
+__device__ __forceinline__ void cluster_sums(float4 (&sums)[SUM_ROWS], uint32_t result, int lane, int skipped, int parts, int first, int step, int end,
+                                             Weight weight) {
+    constexpr int AT_ONCE = 4;
+#pragma unroll
+    for (int k = 0; k < SUM_ROWS; ++k) {
+        sums[k] = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+    }
+#pragma unroll 1
+    for (int base = skipped; base < parts; base += AT_ONCE) {
+        float4 x[AT_ONCE][SUM_ROWS];
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) {
+            const uint32_t from = sm100::map_to_cta(result, min(base + n, parts - 1));
+#pragma unroll
+            for (int k = 0; k < SUM_ROWS; ++k) {
+                x[n][k] = base + n < parts && first + k * step < end ? cluster_load4(from + result_unit(first + k * step, lane)) : make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+            }
+        }
+#pragma unroll
+        for (int n = 0; n < AT_ONCE; ++n) {
+#pragma unroll
+            for (int k = 0; k < SUM_ROWS; ++k) {
+                const float w = weight(k, min(base + n, parts - 1));
+                sums[k] = make_float4(fmaf(w, x[n][k].x, sums[k].x), fmaf(w, x[n][k].y, sums[k].y), fmaf(w, x[n][k].z, sums[k].z), fmaf(w, x[n][k].w, sums[k].w));
+            }
+        }
+    }
 }
 
 }  // namespace dscuda

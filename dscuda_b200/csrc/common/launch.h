@@ -18,23 +18,34 @@ namespace dscuda {
 // life begins before the grid in front has ended.  No kernel lets its dependents go early
 // (griddepcontrol.launch_dependents): blocks of the next grid that sit beside a running decode slowed it (8 ragged sequences,
 // 128 heads: 35.3 us without, 41-44 us with), and nothing else gained.
+// `cluster`: consecutive blocks (in x) that make a cluster; 1 for none.
 template <class... Parameters, class... Arguments>
-void launch_chained(void (*kernel)(Parameters...), dim3 grid, dim3 block, std::size_t shared_bytes, cudaStream_t stream, Arguments&&... arguments) {
-    cudaLaunchAttribute attribute{};
-    attribute.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attribute.val.programmaticStreamSerializationAllowed = 1;
+void launch_chained_clusters(void (*kernel)(Parameters...), dim3 grid, unsigned cluster, dim3 block, std::size_t shared_bytes, cudaStream_t stream,
+                             Arguments&&... arguments) {
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = cluster;
+    attributes[1].val.clusterDim.y = 1;
+    attributes[1].val.clusterDim.z = 1;
     cudaLaunchConfig_t config{};
     config.gridDim = grid;
     config.blockDim = block;
     config.dynamicSmemBytes = shared_bytes;
     config.stream = stream;
-    config.attrs = &attribute;
-    config.numAttrs = 1;
+    config.attrs = attributes;
+    config.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t result = cudaLaunchKernelEx(&config, kernel, std::forward<Arguments>(arguments)...);
     if (result != cudaSuccess) {
         (void)cudaGetLastError();       // reported here: the caller's next check must not find it again
     }
     CUDA_CHECK(result);
+}
+
+template <class... Parameters, class... Arguments>
+void launch_chained(void (*kernel)(Parameters...), dim3 grid, dim3 block, std::size_t shared_bytes, cudaStream_t stream, Arguments&&... arguments) {
+    launch_chained_clusters(kernel, grid, 1, block, shared_bytes, stream, std::forward<Arguments>(arguments)...);
 }
 
 }  // namespace dscuda
