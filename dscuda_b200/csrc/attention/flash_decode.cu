@@ -81,6 +81,7 @@ struct DecodeParams {
     float* part_lse;                    // [2 * MOST_CTAS][rows of a block], log2 domain
     PartNote* notes;                    // [B][items]
     int batch, tokens, heads, kv_heads, group;
+    unsigned group_inverse;             // ceil(2^32 / group), 0 for a group of 1
     int page, pages, blocks;
     int keys_most;                      // pages * page, or Tk
     int row_blocks;
@@ -183,14 +184,19 @@ __device__ __forceinline__ unsigned item_cost(int length, int tile) {
     return length > 0 ? (length + tile - 1) / tile + ITEM_TILES : 0;
 }
 
+// row / group: exact for row * group < 2^32 (a row is below 64 * group, a group at most 4096).
+__device__ __forceinline__ int token_of(const DecodeParams& p, int row) {
+    return p.group_inverse == 0 ? row : static_cast<int>(__umulhi(static_cast<unsigned>(row), p.group_inverse));
+}
+
 // The address of a query or output row: row = token * group + head of the group.
 __device__ __forceinline__ size_t row_offset(const DecodeParams& p, int b, int kv_head, int row) {
-    const int token = row / p.group;
+    const int token = token_of(p, row);
     return ((static_cast<size_t>(b) * p.tokens + token) * p.heads + kv_head * p.group + (row - token * p.group)) * HEAD;
 }
 
 __device__ __forceinline__ size_t lse_offset(const DecodeParams& p, int b, int kv_head, int row) {
-    const int token = row / p.group;
+    const int token = token_of(p, row);
     return (static_cast<size_t>(b) * p.heads + kv_head * p.group + (row - token * p.group)) * p.tokens + token;
 }
 
@@ -290,6 +296,19 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
         const int row_base = (static_cast<int>(item) - kv_head * p.row_blocks) * S::ROWS;
         const int rows = p.group * p.tokens;
 
+        // ---- Q on its way, in front of the keys in the queue of the memory: lane (g, c) has row g of each block of 8 ------------
+        uint4 raw[NB][4];
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb) {
+            const int row = row_base + nb * 8 + g;
+            const uint4* src = reinterpret_cast<const uint4*>(p.query + (row < rows ? row_offset(p, entry, kv_head, row) : 0));
+            // 8-bit: k-step 4 j + i holds columns 16 (c + 4 j) + 4 i .. + 3; bf16: k-step 2 j + i columns 8 (c + 4 j) + 4 i .. + 3
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                raw[nb][u] = row < rows ? src[SOURCE == BF16 ? c + 4 * u : 2 * (c + 4 * (u / 2)) + u % 2] : make_uint4(0, 0, 0, 0);
+            }
+        }
+
         // ---- the warp's keys: steps of KEYS, one to a tile ------------------------------------------------
         const int first_key = tile_begin * S::TILE + warp * KEYS;
         const int steps = min(tile_end - tile_begin, max(0, (length - first_key + S::TILE - 1) / S::TILE));
@@ -368,32 +387,27 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
             issue(s);
         }
 
-        // ---- Q: B fragments in the column order of the codes; lane (g, c) has row g of each block ----------------
+        // ---- Q: B fragments in the column order of the codes ----------------
         uint2 query[QUERY_IN_REGISTERS ? NB : 1][KSTEPS];
         float factor[NB][2];            // scale * log2(e) * 2^-shift of rows 2 c and 2 c + 1
         int limit[NB][2];               // keys that they see
         int least = 0x7fffffff;         // the fewest that a row sees
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
-            const int row = row_base + nb * 8 + g;
-            const uint4* src = reinterpret_cast<const uint4*>(p.query + (row < rows ? row_offset(p, entry, kv_head, row) : 0));
-            uint32_t raw[KSTEPS * 2];
-            // 8-bit: k-step 4 j + i holds columns 16 (c + 4 j) + 4 i .. + 3; bf16: k-step 2 j + i columns 8 (c + 4 j) + 4 i .. + 3
+            uint32_t pairs[KSTEPS * 2];
 #pragma unroll
             for (int u = 0; u < 4; ++u) {
-                const int unit = SOURCE == BF16 ? c + 4 * u : 2 * (c + 4 * (u / 2)) + u % 2;
-                const uint4 v = row < rows ? src[unit] : make_uint4(0, 0, 0, 0);
-                raw[4 * u] = v.x;
-                raw[4 * u + 1] = v.y;
-                raw[4 * u + 2] = v.z;
-                raw[4 * u + 3] = v.w;
+                pairs[4 * u] = raw[nb][u].x;
+                pairs[4 * u + 1] = raw[nb][u].y;
+                pairs[4 * u + 2] = raw[nb][u].z;
+                pairs[4 * u + 3] = raw[nb][u].w;
             }
             float down = p.scale * LOG2E;
             if (SOURCE != BF16) {
                 float largest = 0.0F;
 #pragma unroll
                 for (int e = 0; e < KSTEPS * 2; ++e) {
-                    largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(raw[e] << 16)), fabsf(__uint_as_float(raw[e] & 0xffff0000U))));
+                    largest = fmaxf(largest, fmaxf(fabsf(__uint_as_float(pairs[e] << 16)), fabsf(__uint_as_float(pairs[e] & 0xffff0000U))));
                 }
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffU, largest, 1));
                 largest = fmaxf(largest, __shfl_xor_sync(0xffffffffU, largest, 2));
@@ -403,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                 down *= __uint_as_float(static_cast<uint32_t>(127 - shift) << 23);
 #pragma unroll
                 for (int e = 0; e < KSTEPS * 2; ++e) {
-                    raw[e] = pack_f16x2(__uint_as_float(raw[e] << 16) * up, __uint_as_float(raw[e] & 0xffff0000U) * up);
+                    pairs[e] = pack_f16x2(__uint_as_float(pairs[e] << 16) * up, __uint_as_float(pairs[e] & 0xffff0000U) * up);
                 }
             }
 #pragma unroll
@@ -411,15 +425,15 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                 const int column = row_base + nb * 8 + 2 * c + side;
                 factor[nb][side] = __shfl_sync(0xffffffffU, down, 8 * c + 4 * side);
                 // (rows that do not exist have Q = 0 and are not written)
-                limit[nb][side] = p.causal && column < rows ? length - p.tokens + 1 + column / p.group : length;
+                limit[nb][side] = p.causal && column < rows ? length - p.tokens + 1 + token_of(p, column) : length;
                 least = min(least, limit[nb][side]);
             }
 #pragma unroll
             for (int k = 0; k < KSTEPS; ++k) {
                 if constexpr (QUERY_IN_REGISTERS) {
-                    query[nb][k] = make_uint2(raw[2 * k], raw[2 * k + 1]);
+                    query[nb][k] = make_uint2(pairs[2 * k], pairs[2 * k + 1]);
                 } else if (warp == nb % WARPS) {
-                    *reinterpret_cast<uint2*>(smem + S::RING + ((nb * KSTEPS + k) * 32 + lane) * 8) = make_uint2(raw[2 * k], raw[2 * k + 1]);
+                    *reinterpret_cast<uint2*>(smem + S::RING + ((nb * KSTEPS + k) * 32 + lane) * 8) = make_uint2(pairs[2 * k], pairs[2 * k + 1]);
                 }
             }
         }
@@ -832,6 +846,10 @@ void launch_decode(DecodeParams& p, cudaStream_t stream) {
         }
     }
     const int rows = p.group * p.tokens;
+    if (p.group > 4096) {
+        throw std::invalid_argument("flash attention over few rows takes at most 4096 query heads to a key head");
+    }
+    p.group_inverse = p.group == 1 ? 0 : static_cast<unsigned>(((1ULL << 32) + p.group - 1) / p.group);
     p.row_blocks = (rows + S::ROWS - 1) / S::ROWS;
     const long long most = static_cast<long long>((p.keys_most + S::TILE - 1) / S::TILE + ITEM_TILES) * p.batch * p.kv_heads * p.row_blocks;
     if (most > 0x7fffffffLL) {
