@@ -154,7 +154,8 @@ def decode_and_compare(gpu, kind, lengths, tokens, hq, hkv, page, seed, pages=No
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("lengths,tokens,hq,hkv,page", [
     ([1], 1, 1, 1, 16), ([700], 1, 32, 8, 64), ([0, 1, 15, 16, 17, 31, 32, 33, 127, 128, 129], 1, 8, 2, 16), ([64, 65, 63, 500], 1, 16, 1, 32),
-    ([300, 5, 1, 0], 4, 12, 4, 64), ([1000, 129], 2, 32, 2, 128), ([90, 4000], 8, 28, 4, 64), ([40, 64, 65], 64, 3, 1, 48), ([2500, 17], 3, 5, 5, 144),
+    ([300, 5, 1, 0], 4, 12, 4, 64), ([1000, 129], 2, 32, 2, 128), ([700, 128, 0, 129, 1, 3000], 8, 32, 2, 64), ([640, 20], 17, 1, 1, 16), ([2000, 33, 256], 5, 24, 2, 32),
+    ([513, 64], 64, 4, 1, 128), ([400], 9, 130, 2, 48), ([90, 4000], 8, 28, 4, 64), ([40, 64, 65], 64, 3, 1, 48), ([2500, 17], 3, 5, 5, 144),
 ])
 def test_decode(gpu, kind, lengths, tokens, hq, hkv, page):
     decode_and_compare(gpu, kind, lengths, tokens, hq, hkv, page, 20 + tokens)
@@ -164,6 +165,8 @@ def test_decode_long_and_many(gpu):
     decode_and_compare(gpu, torch.int8, [70001], 1, 8, 2, 64, 31)
     decode_and_compare(gpu, torch.float8_e4m3fn, [3 + 37 * i % 900 for i in range(200)], 1, 8, 4, 64, 32)
     decode_and_compare(gpu, torch.int8, [9000] + [0] * 140 + [1] * 20, 1, 4, 4, 32, 33)
+    decode_and_compare(gpu, torch.float8_e4m3fn, [5 + 53 * i % 700 for i in range(90)], 5, 16, 4, 32, 34)
+    decode_and_compare(gpu, torch.int8, [30000, 0, 70, 15000], 8, 8, 2, 64, 35)
 
 
 def test_lengths_behind_the_table_and_large_queries(gpu):
