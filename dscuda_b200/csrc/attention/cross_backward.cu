@@ -19,7 +19,7 @@
 // back, moves 4 bytes per pair through HBM, 0.62 ps at the measured copy rate, against 0.31 ps for the 512 FLOP at the measured tensor rate.
 //
 // Every gradient element has one writer and a fixed order of sums: results are the same bits from call to call.  P and dS are rounded to
-// bf16 (half a step is 2^-9); everything else is fp32.
+// bf16 (half a step is 2^-8); everything else is fp32.
 //
 // Rows that do not exist (a group that does not divide 64, tokens behind the last) carry lse = +inf, which makes their P zero, and zeros for Q and
 // dO.  Keys behind an entry's length cost nothing in the key kernel (one thread owns a key, its sums are replaced by zeros at the end); the

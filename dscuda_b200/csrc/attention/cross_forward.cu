@@ -16,7 +16,7 @@
 //
 // Few rows to a key head (single tokens) go to flash_decode.cu instead, which splits the keys over the SMs.
 //
-// P is rounded to bf16 (half a step is 2^-9 of each weight); sums, maxima and O are fp32.  Every wait is bounded.
+// P is rounded to bf16 (half a step is 2^-8 of each weight); sums, maxima and O are fp32.  Every wait is bounded.
 #include "flash_attention.h"
 #include "cuda_common.h"
 #include "attention_internal.h"

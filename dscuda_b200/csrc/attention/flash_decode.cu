@@ -4,13 +4,18 @@
 //     for each page and head;
 //   * over an encoder's states in bf16, [B, Tk, Hkv, 128], each entry with its own length.
 //
-// The rows of one key/value head are its group's heads times the new tokens (row = token * group + head), in blocks of 16 or 32,
-// so a key is fetched once for all of them.  Per key x and row r: s = scale * ks * (q . x), online softmax, O += p * vs * v.
+// The rows of one key/value head are its group's heads times the new tokens (row = token * group + head), in blocks of 8, 16 or 32,
+// so a key is fetched once for a block.  Per key x and row r: s = scale * ks * (q . x), online softmax, O += p * vs * v.
 //
 // Bound: HBM, 256 bytes per cached token and head (8 bits) against 4 * 128 FLOP per row.  With 16 rows that is 32 FLOP per byte,
 // far below the tensor core's ratio, so the products run on mma.sync (m16n8k16, fp32 sums): 16 rows fit its tile, its operands
-// come from registers where the codes are widened on the way, and at the copy rate it is a third busy.  tcgen05 would want
-// 128 rows and the widened tile written back to shared memory.
+// come from registers where the codes are widened on the way, and at the copy rate it is a third busy.  tcgen05 wants the
+// widened tile written back to shared memory, 192 KB of traffic a tile: measured over 8 sequences of 20000-40000 positions it took 140 us for 32
+// rows (this form 116) and 154 for 64 (213: the cache is read twice), over 32 sequences of 500-4000 114 us for 64 rows (96).  Steps of single
+// tokens and short drafts are what this is for, so the one form serves all.
+//
+// Measured (64 query heads on 8): 32 sequences of 1000-8000 tokens 46.5 us (floor 38.3), 4 drafted tokens at 20000-40000 120 us (floor
+// 72.7; bound by the issue of widening and softmax beside the copies), one sequence of 100 tokens 8.3 us (two launches).
 //
 // Operands.  Codes become f16 (exact for both types: int8 through 1024 + u - 1152, e4m3 by conversion) and so does Q, each row
 // multiplied by a power of two that brings its largest element to 2^13..2^14; P is rounded to f16 (half a step is 2^-11 of it), relative to the
@@ -19,7 +24,7 @@
 //
 // Products.  S^T = K Q^T and O^T = V^T P^T: the keys, and then the head columns, are the 16 rows of an instruction, the query rows its 8
 // columns, so that 1 to 8 query rows waste nothing (with the rows on the 16-row side a step of four heads took twice the tensor instructions and
-// twice the softmax: 74 us for 32 ragged sequences where this form takes FIGURE).  The 8 x 8 blocks of P^T are turned by movmatrix.
+// twice the softmax: 74 us for 32 ragged sequences where this form took 52).  The 8 x 8 blocks of P^T are turned by movmatrix.
 // The order of head columns inside a product is free as long as both factors agree, so a thread takes 16 consecutive bytes of a key
 // (four k-steps of its fragment) instead of a gather, and of a value 16 consecutive bytes of four keys.  Rows in shared memory are
 // swizzled by ((r & 7) >> 1) | ((r & 1) << 2) in 16-byte units, which makes both read patterns free of bank conflicts.
@@ -541,8 +546,6 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
                     value_scale[u] = meta.value[u] * inverse;
                 }
             }
-            // The reference m of a row lags its maximum by up to the threshold: the lanes of a row compare notes, and the sums are rescaled,
-            // only when one of them passes it.
             // x = score * f - reference for the pair of query rows at once.  The reference m of a row lags its maximum by up to the threshold: the
             // lanes of a row compare notes, and the sums are rescaled, only when one of them passes it.
             float2 f[KU][NB];
@@ -836,15 +839,6 @@ int blocks_of_rows(long long rows) {
 template <int SOURCE, int NB>
 void launch_decode(DecodeParams& p, cudaStream_t stream) {
     using S = Shape<SOURCE, NB>;
-    static bool done[16] = {};
-    int device = 0;
-    CUDA_CHECK(cudaGetDevice(&device));
-    if (device >= 16 || !done[device]) {
-        CUDA_CHECK(cudaFuncSetAttribute(flash_decode_kernel<SOURCE, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
-        if (device < 16) {
-            done[device] = true;
-        }
-    }
     const int rows = p.group * p.tokens;
     if (p.group > 4096) {
         throw std::invalid_argument("flash attention over few rows takes at most 4096 query heads to a key head");
@@ -854,6 +848,15 @@ void launch_decode(DecodeParams& p, cudaStream_t stream) {
     const long long most = static_cast<long long>((p.keys_most + S::TILE - 1) / S::TILE + ITEM_TILES) * p.batch * p.kv_heads * p.row_blocks;
     if (most > 0x7fffffffLL) {
         throw std::invalid_argument("flash attention over few rows: the shape exceeds the supported index range");
+    }
+    static bool done[16] = {};
+    int device = 0;
+    CUDA_CHECK(cudaGetDevice(&device));
+    if (device >= 16 || !done[device]) {
+        CUDA_CHECK(cudaFuncSetAttribute(flash_decode_kernel<SOURCE, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::BYTES));
+        if (device < 16) {
+            done[device] = true;
+        }
     }
     const int ctas = static_cast<int>(std::min<long long>(148LL * S::CTAS_PER_SM, most));
     p.part_lse = p.part_out + static_cast<size_t>(2 * MOST_CTAS) * S::ROWS * HEAD;

@@ -656,7 +656,8 @@ DSCUDA_FUNCTION(flash_rope) {
         }
         std::vector<int> sections;
         for (Py_ssize_t i = 0; i < PySequence_Fast_GET_SIZE(items.get()); ++i) {
-            sections.push_back(static_cast<int>(integer(PySequence_Fast_GET_ITEM(items.get(), i))));
+            const long long pairs = integer(PySequence_Fast_GET_ITEM(items.get(), i));
+            sections.push_back(pairs >= 0 && pairs <= width ? static_cast<int>(pairs) : 0);     // (0 is refused)
         }
         const Tensor& positions = tensor(args[2]);
         if (positions.device() != anchor->device() || positions.scalar_type() != at::kInt) {
@@ -667,18 +668,19 @@ DSCUDA_FUNCTION(flash_rope) {
         }
         const float theta = number(args[4]);
         const bool restart = truth(args[5]), inverse = truth(args[6]);
-        Tensor made[2];
         for (int i = 0; i < 2; ++i) {
-            if (in[i].tensor == nullptr) {
-                if (args[7 + i] != Py_None) {
-                    fail(PyExc_ValueError, std::string(names[i]) + " is missing, but its output is given");
-                }
+            if (args[7 + i] == Py_None) {
                 continue;
             }
-            if (args[7 + i] != Py_None) {
-                out[i] = strided_rows(args[7 + i], "an output");
-                expect_input(*out[i].tensor, *anchor, at::kBFloat16, in[i].tensor->sizes(), "an output");
-            } else {
+            if (in[i].tensor == nullptr) {
+                fail(PyExc_ValueError, std::string(names[i]) + " is missing, but its output is given");
+            }
+            out[i] = strided_rows(args[7 + i], "an output");
+            expect_input(*out[i].tensor, *anchor, at::kBFloat16, in[i].tensor->sizes(), "an output");
+        }
+        Tensor made[2];
+        for (int i = 0; i < 2; ++i) {
+            if (in[i].tensor != nullptr && out[i].tensor == nullptr) {
                 made[i] = new_tensor(in[i].tensor->sizes(), *anchor, at::kBFloat16);
                 out[i] = {&made[i], made[i].size(-2) * made[i].size(-1)};
             }

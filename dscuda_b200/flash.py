@@ -36,9 +36,9 @@ def cache_append(key_cache, value_cache, key_scale, value_scale, key, value, blo
     key_cache, value_cache [blocks, Hkv, page, 128] int8 or float8_e4m3fn (page a multiple of 16), key_scale, value_scale [blocks, Hkv]
     fp32; key, value [B, T, Hkv, 128], tokens may lie apart; block_table [B, pages] int32; start_positions / token_counts [B] int32 or None
     (0 / all T tokens).  Token t of sequence b lands at position start_positions[b] + t.
-    A page's scale covers what the page holds: where new values need a larger one, the page's older codes are rounded again.  A page must
-    not be written for two sequences in one call.  Positions and page numbers outside the cache are skipped and raise
-    status 3 (`device_status`)."""
+    A page's scale covers what the page holds: where new values need a larger one, the page's older codes are rounded again.  What
+    a sequence held at and behind its first new position is given up.  A page must not be written twice in one call (two sequences that share it have
+    to part before).  Positions and page numbers outside the cache are skipped and raise status 3 (`device_status`)."""
     extension().flash_cache_append(key_cache, value_cache, key_scale, value_scale, key, value, block_table, start_positions, token_counts)
 
 

@@ -62,7 +62,7 @@ void flash_rope_cuda(
     cudaStream_t stream = nullptr);
 
 // The paged cache in 8 bits: keys and values each as codes [cache_blocks, Hkv, page_size, 128] with one FP32 scale for each page and
-// head, [cache_blocks, Hkv]; value = code * scale, scales are not negative.  page_size is a multiple of 16.
+// head, [cache_blocks, Hkv]; value = code * scale, with the scales that flash_cache_append_cuda writes.  page_size is a multiple of 16.
 enum class FlashCacheType : int {
     INT8 = 0,           // codes -127..127
     E4M3 = 1,           // codes up to +-448
@@ -76,8 +76,9 @@ constexpr int FLASH_DECODE_MAX_TOKENS = 64;
 // A page's scale covers the values it holds: need = max|new| * (1/127 or 1/448 as FP32), or 0 when that maximum is below 2^-100; a page that starts
 // with a new token takes `need`, another max(its scale, need), and where that raises the scale its older codes are rounded again to
 // the new one.  code = round-half-even(x * (1 / scale)).  NaN becomes 0, an infinity the largest code; neither counts for the scale.
-// A page must not be written for two sequences in one call.  A position or page number outside the cache is not written and
-// sets the device status to 3.
+// What a page held at and behind the first new position is given up, whether it is written over or not (its codes do not follow the scale).  A
+// page must not be written twice in one call, for two sequences or for one.  A position or page number outside the cache is not written
+// and sets the device status to 3.
 void flash_cache_append_cuda(
     void* key_cache,
     void* value_cache,
