@@ -9,6 +9,7 @@
 #include "dscuda_c_api.h"
 
 #include <ATen/Functions.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -163,12 +164,13 @@ void* current_stream() {
     return c10::cuda::getCurrentCUDAStream().stream();
 }
 
+// Straight from the CUDA allocator: through the dispatcher each output of a small call costs 0.6 us more (flash_rope with two: 5.9 us, so 4.7).
 Tensor new_tensor(at::IntArrayRef sizes, const Tensor& like, at::ScalarType type) {
-    return at::empty(sizes, at::TensorOptions().device(like.device()).dtype(type));
+    return at::detail::empty_cuda(sizes, type, like.device(), std::nullopt);
 }
 
 Tensor new_like(const Tensor& t) {
-    return at::empty(t.sizes(), at::TensorOptions().device(t.device()).dtype(t.scalar_type()));
+    return new_tensor(t.sizes(), t, t.scalar_type());
 }
 
 // The interpreter lock is released for the lifetime of this object; taken back when an exception passes too (data_ptr() of a
