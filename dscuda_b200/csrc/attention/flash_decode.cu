@@ -760,11 +760,18 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
     }
 }
 
-// Joins the parts of the items that several CTAs worked on, in the order of their keys, and writes the rows of entries without any key.  A
-// warp takes a row, a lane four of its columns.
+// Joins the parts of the items that several CTAs worked on, in the order of their keys, and writes the rows of entries without any key.  SHARE
+// warps take a row, a lane four of its columns; each warp joins a run of the row's parts, four (eight) of them on the way at once, and the
+// first one joins the runs.  One warp to a row joined the 58 parts of 2 x 8 rows over 7354 keys (two kernels) in 15.4 us, four
+// join them in 7.6.
+template <int SHARE>
 __global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __grid_constant__ DecodeParams p, int block_rows) {
+    static_assert(SHARE == 1 || SHARE == WARPS, "a warp or a CTA to a row");
+    __shared__ float4 run_value[SHARE > 1 ? WARPS : 1][32];
+    __shared__ float2 run_sum[WARPS];                               // reference (log2 domain) and sum of a warp's run
     const int rows = p.group * p.tokens;
-    const int index = blockIdx.x * WARPS + threadIdx.x / 32;        // kv_head * rows + row
+    const int warp = threadIdx.x / 32;
+    const int index = SHARE == 1 ? blockIdx.x * WARPS + warp : blockIdx.x;      // kv_head * rows + row
     const int lane = threadIdx.x % 32;
     const int entry = blockIdx.y;
     if (index >= p.kv_heads * rows) {
@@ -779,9 +786,11 @@ __global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __g
     uint2* out = reinterpret_cast<uint2*>(p.out + row_offset(p, entry, kv_head, row)) + lane;
     float* lse = p.lse + lse_offset(p, entry, kv_head, row);
     if (length == 0) {
-        *out = make_uint2(0, 0);
-        if (lane == 0) {
-            *lse = -INFINITY;
+        if (SHARE == 1 || warp == 0) {
+            *out = make_uint2(0, 0);
+            if (lane == 0) {
+                *lse = -INFINITY;
+            }
         }
         return;
     }
@@ -793,23 +802,24 @@ __global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __g
     auto slot_row = [&](int part) {
         return static_cast<size_t>(2 * (note.first + part) + (part == 0 ? note.count_slot % 2 : 0)) * block_rows + inside;
     };
-    // one pass, four parts at a time: their logarithms and columns are on the way together
-    constexpr int AT_ONCE = 4;
+    // one pass, some parts at a time: their logarithms and columns are on the way together
+    constexpr int AT_ONCE = SHARE == 1 ? 4 : 8;
+    const int begin = SHARE == 1 ? 0 : count * warp / SHARE, end = SHARE == 1 ? count : count * (warp + 1) / SHARE;
     float top = -INFINITY, sum = 0.0F;
     float4 value = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
-    for (int base = 0; base < count; base += AT_ONCE) {
+    for (int base = begin; base < end; base += AT_ONCE) {
         float lse2[AT_ONCE];
         float4 x[AT_ONCE];
 #pragma unroll
         for (int n = 0; n < AT_ONCE; ++n) {
-            const size_t at = slot_row(min(base + n, count - 1));
+            const size_t at = slot_row(min(base + n, end - 1));
             lse2[n] = p.part_lse[at];
             x[n] = *reinterpret_cast<const float4*>(p.part_out + at * HEAD + lane * 4);
         }
         float now = top;
 #pragma unroll
         for (int n = 0; n < AT_ONCE; ++n) {
-            lse2[n] = base + n < count ? lse2[n] : -INFINITY;
+            lse2[n] = base + n < end ? lse2[n] : -INFINITY;
             now = fmaxf(now, lse2[n]);
         }
         const float reference = now == -INFINITY ? 0.0F : now;
@@ -824,12 +834,42 @@ __global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __g
         }
         top = now;
     }
+    if constexpr (SHARE > 1) {
+        run_value[warp][lane] = value;
+        if (lane == 0) {
+            run_sum[warp] = make_float2(top, sum);
+        }
+        __syncthreads();
+        if (warp != 0) {
+            return;
+        }
+        float now = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < SHARE; ++w) {
+            now = fmaxf(now, run_sum[w].x);
+        }
+        const float reference = now == -INFINITY ? 0.0F : now;
+        sum = 0.0F;
+        value = make_float4(0.0F, 0.0F, 0.0F, 0.0F);
+#pragma unroll
+        for (int w = 0; w < SHARE; ++w) {
+            const float weight = exp2_approx(run_sum[w].x - reference);
+            const float4 x = run_value[w][lane];
+            sum = fmaf(weight, run_sum[w].y, sum);
+            value = make_float4(fmaf(weight, x.x, value.x), fmaf(weight, x.y, value.y), fmaf(weight, x.z, value.z), fmaf(weight, x.w, value.w));
+        }
+        top = now;
+    }
     const float inverse = sum == 0.0F ? 0.0F : 1.0F / sum;
     *out = make_uint2(sm100::pack_bf16x2(value.x * inverse, value.y * inverse), sm100::pack_bf16x2(value.z * inverse, value.w * inverse));
     if (lane == 0) {
         *lse = sum == 0.0F ? -INFINITY : (top + log2f(sum)) * LN2;
     }
 }
+
+// Rows up to which each has a CTA of the joining kernel.  Both kernels with a warp and a CTA to a row: 8 rows over 40000 keys 52.3 and 15.8 us, 128 over
+// 3000 12.6 and 10.2, 1024 over 5000 21.8 and 22.1, 2048 over 600 14.8 and 16.8.
+constexpr long long WIDE_COMBINE_ROWS = 512;
 
 // Blocks of 8 query rows that an item has.
 int blocks_of_rows(long long rows) {
@@ -862,7 +902,11 @@ void launch_decode(DecodeParams& p, cudaStream_t stream) {
     p.part_lse = p.part_out + static_cast<size_t>(2 * MOST_CTAS) * S::ROWS * HEAD;
     p.notes = reinterpret_cast<PartNote*>(p.part_lse + static_cast<size_t>(2 * MOST_CTAS) * S::ROWS);
     launch_chained(flash_decode_kernel<SOURCE, NB>, dim3(ctas), dim3(THREADS), S::BYTES, stream, p);
-    launch_chained(flash_decode_combine_kernel, dim3((p.kv_heads * rows + WARPS - 1) / WARPS, p.batch), dim3(THREADS), 0, stream, p, S::ROWS);
+    if (static_cast<long long>(p.kv_heads) * rows * p.batch <= WIDE_COMBINE_ROWS) {
+        launch_chained(flash_decode_combine_kernel<WARPS>, dim3(p.kv_heads * rows, p.batch), dim3(THREADS), 0, stream, p, S::ROWS);
+    } else {
+        launch_chained(flash_decode_combine_kernel<1>, dim3((p.kv_heads * rows + WARPS - 1) / WARPS, p.batch), dim3(THREADS), 0, stream, p, S::ROWS);
+    }
 }
 
 template <int SOURCE>

@@ -21,13 +21,17 @@ constexpr int ACTIVE_CLUSTERS[17] = {0, 148, 74, 45, 33, 26, 22, 15, 15, 0, 0, 0
 constexpr double CLUSTER_US = 4.3;
 
 // Parts that a loop of `tiles` tiles of `tile_us` microseconds is cut into when `ctas` whole loops would run: the cluster size (up to `most`: 8 is portable, 16 has
-// to be allowed) of the shortest time, of those of which all clusters run at once.
+// to be allowed) of the shortest time, in as many waves as its clusters need.
 inline int loop_parts(long long ctas, long long tiles, double tile_us, int most) {
     int best = 1;
-    double best_us = static_cast<double>(tiles) * tile_us;
-    for (int parts = 2; parts <= most && parts <= tiles; ++parts) {
-        const double us = static_cast<double>((tiles + parts - 1) / parts) * tile_us + CLUSTER_US;
-        if (ctas <= ACTIVE_CLUSTERS[parts] && us < best_us) {
+    double best_us = 0.0;
+    for (int parts = 1; parts <= most && parts <= tiles; ++parts) {
+        if (ACTIVE_CLUSTERS[parts] == 0) {
+            continue;
+        }
+        const long long waves = (ctas + ACTIVE_CLUSTERS[parts] - 1) / ACTIVE_CLUSTERS[parts];
+        const double us = static_cast<double>(waves) * (static_cast<double>((tiles + parts - 1) / parts) * tile_us + (parts > 1 ? CLUSTER_US : 0.0));
+        if (parts == 1 || us < best_us) {
             best = parts;
             best_us = us;
         }
