@@ -51,6 +51,7 @@ int flash_cache_device_status(bool reset);
 int flash_decode_device_status(bool reset);
 int cross_forward_device_status(bool reset);
 int cross_backward_device_status(bool reset);
+int cross_backward_short_device_status(bool reset);
 
 }  // namespace internal
 }  // namespace dscuda

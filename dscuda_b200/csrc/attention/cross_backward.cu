@@ -28,6 +28,7 @@
 #include "cuda_common.h"
 #include "attention_internal.h"
 #include "sm100_primitives.cuh"
+#include "cross_backward.cuh"
 #include "loop_parts.cuh"
 #include "../common/launch.h"
 #include "../common/tensor_map.h"
@@ -40,56 +41,13 @@
 namespace dscuda {
 namespace {
 
-using namespace sm100;
+using namespace cross;
 
-constexpr int HEAD = 128;
-constexpr int BIG = 128;                    // rows of a resident tile (tensor-memory lanes)
-constexpr int SUB = 64;                     // rows of a streamed query tile
-constexpr int BIG_CHUNK = BIG * 128;        // 16 KB
-constexpr int SUB_CHUNK = SUB * 128;        // 8 KB
-constexpr int THREADS = 320;                // 8 softmax warps, the MMA warp, the load warp
-constexpr int SOFTMAX_THREADS = 256;
-constexpr int MMA_WARP = 8;
-constexpr int LOAD_WARP = 9;
-constexpr int TMEM_COLUMNS = 512;
-constexpr float LOG2E = 1.4426950408889634F;
 constexpr double QUERY_TILE_US = 1.15;      // a key tile of the query kernel's loop
 constexpr double KEY_TILE_US = 0.75;        // a row tile of the key kernel's loop
 constexpr int MOST_KEY_PARTS = 16;          // few keys under many rows: the backward of 64 keys under 4096 x 3 rows 45 us with 8 parts, 38 with 16
 
 __device__ int cross_backward_status = 0;
-
-struct CrossBackwardParams {
-    CUtensorMap q_sub, do_sub;          // group rows, box {64, group, tokens of a 64-row tile}
-    CUtensorMap q_big, do_big, o_big;   // the same for 128-row tiles
-    CUtensorMap k, v;                   // [B][Tk][Hkv * 128], boxes of 128 rows
-    CUtensorMap dq;                     // like q_big
-    CUtensorMap dk, dv;                 // like k
-    float2* rows;                       // [B, Hkv, Tq, group]: lse * log2(e), delta
-    const float* lse;                   // [B, Hq, Tq]
-    const int* lengths;                 // null: Tk
-    __nv_bfloat16 *dq_out, *dk_out, *dv_out;
-    int query_parts, key_parts;         // CTAs (a cluster) that share a loop
-    int tokens, keys, kv_heads, group;
-    int sub_tokens, big_tokens;         // tokens of a query tile of each kind
-    float scale, scale_log2;
-};
-
-__device__ __forceinline__ int length_of(const CrossBackwardParams& p, int entry) {
-    return p.lengths == nullptr ? p.keys : min(max(p.lengths[entry], 0), p.keys);
-}
-
-// Output tiles leave through idle shared memory: thread r lays out its row of 32 columns in the 128-byte-swizzled chunk that a TMA store reads.
-__device__ __forceinline__ void stage_bf16x32(uint8_t* chunk, int r, int half, const uint32_t* values, bool keep) {
-#pragma unroll
-    for (int u = 0; u < 4; ++u) {
-        const uint32_t* x = values + 8 * u;
-        const uint4 vec = keep ? make_uint4(pack_bf16x2(__uint_as_float(x[0]), __uint_as_float(x[1])), pack_bf16x2(__uint_as_float(x[2]), __uint_as_float(x[3])),
-                                            pack_bf16x2(__uint_as_float(x[4]), __uint_as_float(x[5])), pack_bf16x2(__uint_as_float(x[6]), __uint_as_float(x[7])))
-                               : make_uint4(0, 0, 0, 0);
-        *reinterpret_cast<uint4*>(chunk + r * 128 + (((half * 4 + u) ^ (r & 7)) * 16)) = vec;
-    }
-}
 
 // ---------------------------------------------------------------------------
 // dK, dV
@@ -891,6 +849,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
 
 struct Plan {
     int query_parts, key_parts;
+    bool key_short;
 };
 
 Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
@@ -899,7 +858,8 @@ Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
     const long long row_tiles = (queries + BIG / group - 1LL) / (BIG / group);
     const long long sub_tiles = (queries + SUB / group - 1LL) / (SUB / group);
     const long long pairs = static_cast<long long>(batch) * kv_heads;
-    return {loop_parts(row_tiles * pairs, key_tiles, QUERY_TILE_US, 8), loop_parts(key_tiles * pairs, sub_tiles, KEY_TILE_US, MOST_KEY_PARTS)};
+    const int key_parts = loop_parts(key_tiles * pairs, sub_tiles, KEY_TILE_US, MOST_KEY_PARTS);
+    return {loop_parts(row_tiles * pairs, key_tiles, QUERY_TILE_US, 8), key_parts, key_parts == 1 && cross_key_short_takes(key_tiles * pairs, sub_tiles)};
 }
 
 void configure() {
@@ -969,6 +929,9 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     p.v = make_bf16_batched_tile_map(value, batch_size, key_length, wide, BIG);
     p.dk = make_bf16_batched_tile_map(key_gradient, batch_size, key_length, wide, BIG);
     p.dv = make_bf16_batched_tile_map(value_gradient, batch_size, key_length, wide, BIG);
+    if ((key_length + BIG - 1LL) / BIG * key_value_heads * batch_size > 0x7fffffffLL) {
+        throw std::invalid_argument("flash cross attention shape exceeds the supported index range");
+    }
     const Plan plan = make_plan(batch_size, query_length, key_length, query_heads, key_value_heads);
     p.rows = static_cast<float2*>(workspace);
     p.dq_out = query_gradient;
@@ -983,9 +946,15 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     p.kv_heads = key_value_heads;
     p.scale = scale;
     p.scale_log2 = scale * LOG2E;
+    p.batch = batch_size;
+    p.key_tiles = (key_length + BIG - 1) / BIG;
     configure();
     launch_chained_clusters(cross_query_kernel, dim3((query_length + p.big_tokens - 1) / p.big_tokens * plan.query_parts, key_value_heads, batch_size),
                             plan.query_parts, dim3(THREADS), queryside::SMEM_BYTES, stream, p);
+    if (plan.key_short) {
+        launch_cross_key_short(p, stream);
+        return;
+    }
     launch_chained_clusters(cross_key_kernel, dim3((key_length + BIG - 1) / BIG * plan.key_parts, key_value_heads, batch_size), plan.key_parts, dim3(THREADS),
                             keyside::SMEM_BYTES, stream, p);
 }

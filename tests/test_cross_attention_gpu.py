@@ -57,6 +57,12 @@ SHAPES = [
     (1, 40, 3000, 4, 1, [2900]), (3, 20, 2600, 8, 2, [2600, 100, 0]), (1, 2000, 100, 4, 2, None), (2, 1500, 1030, 3, 1, [1030, 600]), (1, 33, 2049, 1, 1, None),
 ]
 
+# few rows under many keys: CTAs of the key kernel that go over several items
+SHAPES += [
+    (40, 5, 700, 8, 4, [(97 * i) % 701 for i in range(40)]), (2, 12, 5000, 28, 4, [5000, 2500]), (1, 700, 4850, 8, 8, None), (70, 3, 130, 6, 3, [0, 130, 128, 1, 129] * 14),
+    (5, 90, 1100, 12, 12, [0, 0, 0, 0, 1]),
+]
+
 
 @pytest.mark.parametrize("b,tq,tk,hq,hkv,lengths", SHAPES)
 def test_forward_and_gradients(gpu, b, tq, tk, hq, hkv, lengths):
@@ -65,7 +71,7 @@ def test_forward_and_gradients(gpu, b, tq, tk, hq, hkv, lengths):
 
 
 @pytest.mark.parametrize("b,tq,tk,hq,hkv,lengths", [(2, 1, 300, 8, 2, [290, 7]), (3, 77, 333, 6, 2, [300, 0, 128]), (2, 200, 1000, 8, 1, [999, 1]),
-                                                      (2, 20, 2600, 8, 2, [2500, 130])])
+                                                      (2, 20, 2600, 8, 2, [2500, 130]), (40, 5, 700, 8, 4, [(97 * i) % 701 for i in range(40)])])
 def test_padding_is_never_used(gpu, b, tq, tk, hq, hkv, lengths):
     """NaN or infinities behind the lengths: the same bits as zeros there."""
     query, key, value, dout = inputs(gpu, b, tq, tk, hq, hkv)
