@@ -5,14 +5,18 @@
 // of {64 columns, group heads, tokens} lays them out that way (a group that does not divide 128 leaves the last rows of a tile
 // unused).  Short queries fill their tiles and a key tile is fetched once for a whole group.
 //
-// A CTA takes two 128-row tiles of one (entry, key head), which alternate on the tensor core: S = Q K^T into tensor memory, online softmax
-// with one thread to a row, P back into tensor memory as bf16 (P aliases S) and O += P V.  K and V stream through a ring of 16 KB chunks.  Warps
-// 0-3 and 4-7 are the softmax of the two tiles, warp 8 issues the MMAs, warp 9 the loads; warps 10 and 11 clear the value rows behind an
-// entry's length (a weight of zero does not keep their NaN out of P V) and complete the third warpgroup, which hands registers to the
-// softmax.  The schedule is that of prefill_forward.cu, where its measurements stand.
+// A CTA takes one 128-row tile of one (entry, key head): S = Q K^T into tensor memory, online softmax with one thread to a row, P back into tensor memory
+// as bf16 (P aliases S) and O += P V.  It holds half of an SM's tensor memory, shared memory and registers, so that two CTAs share an SM: one's softmax runs
+// beside the other's products, and one's beginning and end beside the other's loop.  (A CTA of two alternating tiles, which fetches K and V
+// once for both, took the same 398 us for the longest case, 4 x 2048 tokens of 32 heads over 2048-4096 keys, but 48.5 for 36.5 on 64 tokens over 1500 keys with 256
+// heads, 29.5 for 22.5 on 584 tokens over 12 keys, 82 for 73 on 835 x 7 rows over 982 ragged keys.)  K and V stream through one tile's place, four chunks of 16 KB: a
+// chunk's successor is on its way as soon as the products that read it are done.
 //
-// Small problems: where pairs of tiles would leave SMs idle a CTA takes one tile, and where that is not enough the loop over the keys is cut into parts
-// for the CTAs of a cluster, which join their fp32 sums through distributed shared memory (loop_parts.cuh).
+// Warps 0-3 are the softmax, warp 4 issues the MMAs, warp 5 the loads; warps 6 and 7 clear the value rows behind an entry's length (a weight of zero
+// does not keep their NaN out of P V).  The second warpgroup hands registers to the softmax, which holds a row of scores.
+//
+// Small problems: where the tiles would leave SMs idle the loop over the keys is cut into parts for the CTAs of a cluster, which join their fp32 sums
+// through distributed shared memory (loop_parts.cuh).
 //
 // Few rows to a key head (single tokens) go to flash_decode.cu instead, which splits the keys over the SMs.
 //
@@ -35,16 +39,15 @@ using namespace sm100;
 constexpr int HEAD = 128;
 constexpr int TILE = 128;                   // rows of a query tile, keys of a key tile
 constexpr int CHUNK = 128 * 128;            // 16 KB: 128 rows x 64 bf16, or 64 keys x 128
-constexpr int RING = 10;
-constexpr int PER_TILE = 4;                 // ring chunks of a key tile: two of K, two of V
-constexpr int Q_BYTES = 4 * CHUNK;
+constexpr int CHUNKS = 4;                   // of a key tile: two of K, two of V
+constexpr int Q_BYTES = 2 * CHUNK;
 constexpr int MISC_BYTES = 2048;
-constexpr int SMEM_BYTES = Q_BYTES + RING * CHUNK + MISC_BYTES + 1024;
-constexpr int THREADS = 384;
-constexpr int MMA_WARP = 8;
-constexpr int LOAD_WARP = 9;
-constexpr int TAIL_WARP = 10;
-constexpr int TMEM_COLUMNS = 512;           // S0 | S1 | O0 | O1
+constexpr int SMEM_BYTES = Q_BYTES + CHUNKS * CHUNK + MISC_BYTES + 1024;
+constexpr int THREADS = 256;
+constexpr int MMA_WARP = 4;
+constexpr int LOAD_WARP = 5;
+constexpr int TAIL_WARP = 6;
+constexpr int TMEM_COLUMNS = 256;           // S | O
 constexpr float RESCALE_THRESHOLD = 8.0F;   // log2 units; below it the old row maximum is kept
 constexpr float LOG2E = 1.4426950408889634F;
 constexpr float LN2 = 0.6931471805599453F;
@@ -61,20 +64,19 @@ struct CrossForwardParams {
     __nv_bfloat16* output;      // [B, Tq, Hq, 128]
     int tokens, keys, heads, group;
     int tile_tokens;            // tokens of a query tile
-    int cta_tiles;              // query tiles of a CTA: 1 or 2
-    int parts;                  // CTAs (a cluster) that share the keys of a query tile; then cta_tiles is 1
+    int parts;                  // CTAs (a cluster) that share the keys of a query tile
     float scale, scale_log2;
 };
 
 struct Barriers {
-    uint64_t q_full[2];
-    uint64_t s_full[2];
-    uint64_t p_full[2];
-    uint64_t p_half[2];
-    uint64_t staged[2];         // the tile's output rows are in shared memory
-    uint64_t ring_full[RING];
-    uint64_t ring_empty[RING];
-    uint64_t tail_full[2];
+    uint64_t q_full;
+    uint64_t s_full;
+    uint64_t p_full;
+    uint64_t p_half;
+    uint64_t staged;            // the output rows are in shared memory
+    uint64_t full[CHUNKS];
+    uint64_t empty[CHUNKS];
+    uint64_t tail_full[2];      // the last tile's value chunks, before the rows behind the length are cleared
     uint32_t tmem_base;
     int abort_flag;
     int gave_up;
@@ -82,35 +84,32 @@ struct Barriers {
 };
 static_assert(sizeof(Barriers) <= MISC_BYTES, "barrier block too large");
 
-__global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_constant__ CrossForwardParams p) {
+__global__ void __launch_bounds__(THREADS, 2) cross_forward_kernel(const __grid_constant__ CrossForwardParams p) {
     extern __shared__ uint8_t smem_raw[];
     const int entry = blockIdx.z;
     const int kv_head = blockIdx.y;
-    const int row_tiles = (p.tokens + p.tile_tokens - 1) / p.tile_tokens;
     const int part = blockIdx.x % p.parts;              // also the rank in the cluster
-    const int tile0 = blockIdx.x / p.parts * p.cta_tiles;
-    const bool second = p.cta_tiles == 2 && tile0 + 1 < row_tiles;
+    const int token0 = blockIdx.x / p.parts * p.tile_tokens;
 
     const uint32_t smem_base = (smem_u32(smem_raw) + 1023U) & ~1023U;
     uint8_t* smem = smem_raw + (smem_base - smem_u32(smem_raw));
-    const uint32_t ring_smem = smem_base + Q_BYTES;
-    Barriers* bars = reinterpret_cast<Barriers*>(smem + Q_BYTES + RING * CHUNK);
+    const uint32_t tile_smem = smem_base + Q_BYTES;
+    Barriers* bars = reinterpret_cast<Barriers*>(smem + Q_BYTES + CHUNKS * CHUNK);
     volatile int* abort_flag = &bars->abort_flag;
     const int warp = threadIdx.x / 32;
     const int lane = threadIdx.x % 32;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < 2; ++i) {
-            mbar_init(smem_u32(&bars->q_full[i]), 1);
-            mbar_init(smem_u32(&bars->s_full[i]), 1);
-            mbar_init(smem_u32(&bars->p_full[i]), TILE);
-            mbar_init(smem_u32(&bars->p_half[i]), TILE);
-            mbar_init(smem_u32(&bars->staged[i]), TILE);
-            mbar_init(smem_u32(&bars->tail_full[i]), 1);
-        }
-        for (int i = 0; i < RING; ++i) {
-            mbar_init(smem_u32(&bars->ring_full[i]), 1);
-            mbar_init(smem_u32(&bars->ring_empty[i]), 1);
+        mbar_init(smem_u32(&bars->q_full), 1);
+        mbar_init(smem_u32(&bars->s_full), 1);
+        mbar_init(smem_u32(&bars->p_full), TILE);
+        mbar_init(smem_u32(&bars->p_half), TILE);
+        mbar_init(smem_u32(&bars->staged), TILE);
+        mbar_init(smem_u32(&bars->tail_full[0]), 1);
+        mbar_init(smem_u32(&bars->tail_full[1]), 1);
+        for (int i = 0; i < CHUNKS; ++i) {
+            mbar_init(smem_u32(&bars->full[i]), 1);
+            mbar_init(smem_u32(&bars->empty[i]), 1);
         }
         bars->abort_flag = 0;
         // after an earlier launch ran into a time limit nothing is done; the CTAs of a cluster stay to the end all the same
@@ -140,72 +139,52 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
     // what lies between the length and the end of the entry's states may be anything; behind that end the loads give zeros
     const int tail_keys = length < p.keys ? min(left - (tile_count - 1) * TILE, TILE) : TILE;
 
-    constexpr int REG_LO = 88;
+    constexpr int REG_LO = 48;
     constexpr int REG_HI = 208;
-    static_assert(8 * (REG_HI - 168) <= 4 * (168 - REG_LO), "register redistribution exceeds the CTA's allocation");
-    if (warp >= 8) {
+    static_assert(4 * REG_HI + 4 * REG_LO <= 8 * 128, "register redistribution exceeds the CTA's allocation");
+    if (warp >= 4) {
         reg_dealloc<REG_LO>();
         if (warp >= TAIL_WARP) {
             if (tail_keys < TILE && tile_count > 0) {
                 const int half = warp - TAIL_WARP;
                 if (__all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->tail_full[half]), 0, abort_flag, &cross_forward_status))) {
-                    const int slot = ((tile_count - 1) * PER_TILE + 2 + half) % RING;
-                    uint8_t* chunk = smem + Q_BYTES + slot * CHUNK;
+                    uint8_t* chunk = smem + Q_BYTES + (2 + half) * CHUNK;
                     const int first = min(max(tail_keys - half * 64, 0), 64);
                     clear_rows(chunk, first, 64, lane);
                     clear_rows(chunk + CHUNK / 2, first, 64, lane);
                     fence_proxy_async_smem();
                     __syncwarp();
                     if (lane == 0) {
-                        mbar_arrive(smem_u32(&bars->ring_full[slot]));
+                        mbar_arrive(smem_u32(&bars->full[2 + half]));
                     }
                 }
             }
         } else if (warp == LOAD_WARP) {
             if (lane == 0 && tile_count > 0) {
-                auto load_q = [&](int i) {
-                    const uint32_t bar = smem_u32(&bars->q_full[i]);
-                    mbar_arrive_expect_tx(bar, 2 * p.group * p.tile_tokens * 128);
-                    for (int c = 0; c < 2; ++c) {
-                        tma_load_4d(smem_base + (2 * i + c) * CHUNK, &p.q, bar, c * 64, kv_head * p.group, (tile0 + i) * p.tile_tokens, entry);
-                    }
-                };
+                const uint32_t q_bar = smem_u32(&bars->q_full);
+                mbar_arrive_expect_tx(q_bar, 2 * p.group * p.tile_tokens * 128);
+                for (int c = 0; c < 2; ++c) {
+                    tma_load_4d(smem_base + c * CHUNK, &p.q, q_bar, c * 64, kv_head * p.group, token0, entry);
+                }
                 bool alive = true;
-                int chunk = 0;
-                auto acquire = [&](uint32_t& bar, uint64_t* counter) -> uint32_t {
-                    const int slot = chunk % RING;
-                    const int use = chunk / RING;
-                    if (use > 0 && !mbar_wait(smem_u32(&bars->ring_empty[slot]), (use - 1) & 1, abort_flag, &cross_forward_status)) {
-                        alive = false;
-                        return 0;
-                    }
-                    bar = smem_u32(counter != nullptr ? counter : &bars->ring_full[slot]);
-                    mbar_arrive_expect_tx(bar, CHUNK);
-                    ++chunk;
-                    return ring_smem + slot * CHUNK;
-                };
-                load_q(0);
 #pragma unroll 1
                 for (int j = 0; j < tile_count && alive; ++j) {
+                    const int key = (first_tile + j) * TILE;
                     const bool tail = tail_keys < TILE && j + 1 == tile_count;
 #pragma unroll 1
-                    for (int c = 0; c < 2 && alive; ++c) {
-                        uint32_t bar;
-                        const uint32_t dst = acquire(bar, nullptr);
-                        if (dst != 0) {
-                            tma_load_3d(dst, &p.k, bar, kv_head * HEAD + c * 64, (first_tile + j) * TILE, entry);
+                    for (int c = 0; c < CHUNKS && alive; ++c) {
+                        if (j > 0 && !mbar_wait(smem_u32(&bars->empty[c]), (j - 1) & 1, abort_flag, &cross_forward_status)) {
+                            alive = false;
+                            break;
                         }
-                    }
-                    if (j == 0 && second) {
-                        load_q(1);
-                    }
-#pragma unroll 1
-                    for (int half = 0; half < 2 && alive; ++half) {
-                        uint32_t bar;
-                        const uint32_t dst = acquire(bar, tail ? &bars->tail_full[half] : nullptr);
-                        if (dst != 0) {
-                            tma_load_3d(dst, &p.v, bar, kv_head * HEAD, (first_tile + j) * TILE + half * 64, entry);
-                            tma_load_3d(dst + CHUNK / 2, &p.v, bar, kv_head * HEAD + 64, (first_tile + j) * TILE + half * 64, entry);
+                        const uint32_t dst = tile_smem + c * CHUNK;
+                        const uint32_t bar = smem_u32(tail && c >= 2 ? &bars->tail_full[c - 2] : &bars->full[c]);
+                        mbar_arrive_expect_tx(bar, CHUNK);
+                        if (c < 2) {
+                            tma_load_3d(dst, &p.k, bar, kv_head * HEAD + c * 64, key, entry);
+                        } else {
+                            tma_load_3d(dst, &p.v, bar, kv_head * HEAD, key + (c - 2) * 64, entry);
+                            tma_load_3d(dst + CHUNK / 2, &p.v, bar, kv_head * HEAD + 64, key + (c - 2) * 64, entry);
                         }
                     }
                 }
@@ -215,98 +194,73 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
             const uint32_t leader = elect_one();
             constexpr uint32_t IDESC_QK = make_idesc_bf16(TILE, TILE, false, false);
             constexpr uint32_t IDESC_PV = make_idesc_bf16(TILE, HEAD, false, true);
-            const int tiles = second ? 2 : 1;
-            bool alive = true;
-            auto wait_chunk = [&](int chunk) -> uint32_t {
-                const int slot = chunk % RING;
-                if (!__all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->ring_full[slot]), (chunk / RING) & 1, abort_flag, &cross_forward_status))) {
-                    alive = false;
-                }
-                return ring_smem + slot * CHUNK;
+            auto wait = [&](uint64_t* barrier, int parity) {
+                return __all_sync(0xffffffffU, mbar_wait(smem_u32(barrier), parity, abort_flag, &cross_forward_status)) != 0;
             };
-            auto issue_qk = [&](int i, int j) {
-                const uint32_t d = tmem_base + i * TILE;
+            auto issue_qk = [&](int j) {
+#pragma unroll
                 for (int c = 0; c < 2; ++c) {
-                    const uint32_t k_chunk = wait_chunk(j * PER_TILE + c);
-                    if (!alive) {
-                        return;
+                    if (!wait(&bars->full[c], j & 1)) {
+                        return false;
                     }
                     tc_fence_after_sync();
-                    const uint32_t q_chunk = smem_base + (2 * i + c) * CHUNK;
+                    const uint32_t q_chunk = smem_base + c * CHUNK, k_chunk = tile_smem + c * CHUNK;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        mma_ss_elect(d, make_kmajor_desc(q_chunk + k * 32), make_kmajor_desc(k_chunk + k * 32), IDESC_QK, (c | k) != 0 ? 1U : 0U, leader);
+                        mma_ss_elect(tmem_base, make_kmajor_desc(q_chunk + k * 32), make_kmajor_desc(k_chunk + k * 32), IDESC_QK,
+                                     (c | k) != 0 ? 1U : 0U, leader);
                     }
                 }
-                mma_commit_elect(smem_u32(&bars->s_full[i]), leader);
-                if (i + 1 == tiles) {
-                    for (int c = 0; c < 2; ++c) {
-                        mma_commit_elect(smem_u32(&bars->ring_empty[(j * PER_TILE + c) % RING]), leader);
-                    }
-                }
+                mma_commit_elect(smem_u32(&bars->s_full), leader);
+                mma_commit_elect(smem_u32(&bars->empty[0]), leader);
+                mma_commit_elect(smem_u32(&bars->empty[1]), leader);
+                return true;
             };
-            auto issue_pv = [&](int i, int j) {
-                const uint32_t d = tmem_base + 2 * TILE + i * HEAD;
-                const uint32_t p_tmem = tmem_base + i * TILE;
+            auto issue_pv = [&](int j) {
+#pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    const uint32_t v_chunk = wait_chunk(j * PER_TILE + 2 + half);
-                    if (alive) {
-                        alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(half == 0 ? &bars->p_half[i] : &bars->p_full[i]), j & 1, abort_flag, &cross_forward_status));
-                    }
-                    if (!alive) {
-                        return;
+                    if (!wait(&bars->full[2 + half], j & 1) || !wait(half == 0 ? &bars->p_half : &bars->p_full, j & 1)) {
+                        return false;
                     }
                     tc_fence_after_sync();
+                    const uint32_t v_chunk = tile_smem + (2 + half) * CHUNK;
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
-                        mma_ts_elect(d, p_tmem + half * 32 + k * 8, make_smem_desc(v_chunk + k * 2048, CHUNK / 2, 1024), IDESC_PV,
+                        mma_ts_elect(tmem_base + TILE, tmem_base + half * 32 + k * 8, make_smem_desc(v_chunk + k * 2048, CHUNK / 2, 1024), IDESC_PV,
                                      (j | half | k) != 0 ? 1U : 0U, leader);
                     }
                 }
-                if (i + 1 == tiles) {
-                    for (int half = 0; half < 2; ++half) {
-                        mma_commit_elect(smem_u32(&bars->ring_empty[(j * PER_TILE + 2 + half) % RING]), leader);
-                    }
-                }
+                mma_commit_elect(smem_u32(&bars->empty[2]), leader);
+                mma_commit_elect(smem_u32(&bars->empty[3]), leader);
+                return true;
             };
-            for (int i = 0; i < tiles && alive; ++i) {
-                alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->q_full[i]), 0, abort_flag, &cross_forward_status));
-                if (alive) {
-                    issue_qk(i, 0);
+            bool alive = wait(&bars->q_full, 0) && issue_qk(0);
+            for (int j = 0; j < tile_count && alive; ++j) {
+                alive = issue_pv(j);
+                if (alive && j + 1 < tile_count) {
+                    alive = issue_qk(j + 1);
                 }
             }
-            for (int j = 0; j < tile_count && alive; ++j) {
-                for (int i = 0; i < tiles && alive; ++i) {
-                    issue_pv(i, j);
-                    if (!alive) {
-                        break;
-                    }
-                    if (j + 1 < tile_count) {
-                        issue_qk(i, j + 1);
-                    } else {
-                        mma_commit_elect(smem_u32(&bars->s_full[i]), leader);       // O_i is final
-                    }
-                }
+            if (alive) {
+                mma_commit_elect(smem_u32(&bars->s_full), leader);      // O is final
             }
         }
     } else {
         // ---- softmax and output: a thread to a row ----
         reg_alloc<REG_HI>();
-        const int i = warp / 4;
         const int r = threadIdx.x % TILE;
         const uint32_t lane_base = static_cast<uint32_t>((warp % 4) * 32) << 16;
-        const uint32_t s_tmem = tmem_base + lane_base + i * TILE;
-        const uint32_t o_tmem = tmem_base + lane_base + 2 * TILE + i * HEAD;
-        const int token = (tile0 + i) * p.tile_tokens + r / p.group;
+        const uint32_t s_tmem = tmem_base + lane_base;
+        const uint32_t o_tmem = tmem_base + lane_base + TILE;
+        const int token = token0 + r / p.group;
         const bool valid = r < p.tile_tokens * p.group && token < p.tokens;
-        const int count = i == 0 || second ? tile_count : 0;
         float* lse = p.lse + (static_cast<size_t>(entry) * p.heads + kv_head * p.group + r % p.group) * p.tokens + token;
         float m_ref = 0.0F;
         float l_sum = 0.0F;
         bool alive = true;
 
-        for (int j = 0; j < count; ++j) {
-            alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->s_full[i]), j & 1, abort_flag, &cross_forward_status));
+        for (int j = 0; j < tile_count; ++j) {
+            alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->s_full), j & 1, abort_flag, &cross_forward_status));
             if (!alive) {
                 break;
             }
@@ -317,7 +271,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
                 tmem_ld_x32(s_tmem + c * 32, sb + c * 32);
             }
             tmem_wait_ld();
-            if (j == count - 1) {
+            if (j == tile_count - 1) {
                 const int present = left - j * TILE;
 #pragma unroll
                 for (int n = 0; n < TILE; ++n) {
@@ -346,7 +300,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
                         m_ref = tile_max;
                         l_sum *= alpha;
                     }
-                    // S_i(j) complete implies P_i(j-1) V complete: O_i is quiescent here
+                    // S(j) complete implies P(j-1) V complete: O is quiescent here
 #pragma unroll
                     for (int c = 0; c < HEAD / 32; ++c) {
                         uint32_t o[32];
@@ -378,37 +332,36 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
                 if (c == 1) {
                     tmem_wait_st();
                     tc_fence_before_sync();
-                    mbar_arrive(smem_u32(&bars->p_half[i]));
+                    mbar_arrive(smem_u32(&bars->p_half));
                 }
             }
             l_sum += sums.x + sums.y;
             tmem_wait_st();
             tc_fence_before_sync();
-            mbar_arrive(smem_u32(&bars->p_full[i]));
+            mbar_arrive(smem_u32(&bars->p_full));
         }
-        const bool active = !dead && (i == 0 || second);
-        if (alive && count > 0) {
-            alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->s_full[i]), count & 1, abort_flag, &cross_forward_status));
+        if (alive && tile_count > 0) {
+            alive = __all_sync(0xffffffffU, mbar_wait(smem_u32(&bars->s_full), tile_count & 1, abort_flag, &cross_forward_status));
         }
-        if (alive && active && p.parts > 1) {
-            // the part's sums into the ring, which is idle by now
+        if (alive && !dead && p.parts > 1) {
+            // the part's sums into the place of K and V, which is idle by now
             tc_fence_after_sync();
 #pragma unroll
-            for (int c = 0; c < HEAD / 32 && count > 0; ++c) {
+            for (int c = 0; c < HEAD / 32 && tile_count > 0; ++c) {
                 uint32_t o[32];
                 tmem_ld_x32(o_tmem + c * 32, o);
                 tmem_wait_ld();
                 result_store32(smem + Q_BYTES, r, c * 32, o);
             }
-            bars->row_sums[r] = count > 0 ? make_float2(m_ref * p.scale_log2, l_sum) : make_float2(-INFINITY, 0.0F);
-        } else if (alive && active) {
-            // rows of 64 columns into the tile's Q chunks (idle by now), from where a TMA store takes them
+            bars->row_sums[r] = tile_count > 0 ? make_float2(m_ref * p.scale_log2, l_sum) : make_float2(-INFINITY, 0.0F);
+        } else if (alive && !dead) {
+            // rows of 64 columns into Q's chunks (idle by now), from where a TMA store takes them
             tc_fence_after_sync();
-            const float inverse = count > 0 ? 1.0F / l_sum : 0.0F;
+            const float inverse = tile_count > 0 ? 1.0F / l_sum : 0.0F;
 #pragma unroll
             for (int c = 0; c < HEAD / 32; ++c) {
                 uint32_t o[32];
-                if (count > 0) {
+                if (tile_count > 0) {
                     tmem_ld_x32(o_tmem + c * 32, o);
                     tmem_wait_ld();
                 } else {
@@ -417,7 +370,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
                         o[e] = 0;
                     }
                 }
-                uint8_t* row = smem + (2 * i + c / 2) * CHUNK + r * 128;
+                uint8_t* row = smem + c / 2 * CHUNK + r * 128;
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
                     uint4 vec;
@@ -429,13 +382,13 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
                 }
             }
             if (valid) {
-                *lse = count > 0 ? m_ref * p.scale + logf(l_sum) : -INFINITY;
+                *lse = tile_count > 0 ? m_ref * p.scale + logf(l_sum) : -INFINITY;
             }
             fence_proxy_async_smem();
-            mbar_arrive(smem_u32(&bars->staged[i]));
-            if (r == 0 && mbar_wait(smem_u32(&bars->staged[i]), 0, abort_flag, &cross_forward_status)) {
+            mbar_arrive(smem_u32(&bars->staged));
+            if (r == 0 && mbar_wait(smem_u32(&bars->staged), 0, abort_flag, &cross_forward_status)) {
                 for (int c = 0; c < 2; ++c) {
-                    tma_store_4d(&p.out, smem_base + (2 * i + c) * CHUNK, c * 64, kv_head * p.group, (tile0 + i) * p.tile_tokens, entry);
+                    tma_store_4d(&p.out, smem_base + c * CHUNK, c * 64, kv_head * p.group, token0, entry);
                 }
                 tma_store_commit();
                 tma_store_wait_read();
@@ -447,7 +400,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
     if (p.parts > 1) {
         __syncwarp();
         cluster_sync_all();
-        const int rows = min(p.tile_tokens, p.tokens - tile0 * p.tile_tokens) * p.group;
+        const int rows = min(p.tile_tokens, p.tokens - token0) * p.group;
         const int row_end = dead ? 0 : part_begin(rows, part + 1, p.parts);
         constexpr int WARPS = THREADS / 32;
         for (int first = part_begin(rows, part, p.parts) + warp; first < row_end; first += SUM_ROWS * WARPS) {
@@ -471,13 +424,13 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
             }
             weight = total == 0.0F ? 0.0F : weight / total;
             float4 value[SUM_ROWS];
-            cluster_sums(value, ring_smem, lane, parts_without(all_tiles, p.parts), p.parts, first, WARPS, row_end,
+            cluster_sums(value, tile_smem, lane, parts_without(all_tiles, p.parts), p.parts, first, WARPS, row_end,
                          [&](int k, int other) { return __shfl_sync(0xffffffffU, weight, 8 * k + other); });
 #pragma unroll
             for (int k = 0; k < SUM_ROWS; ++k) {
                 const int row = first + k * WARPS;
                 if (row < row_end) {
-                    const int token = tile0 * p.tile_tokens + row / p.group;
+                    const int token = token0 + row / p.group;
                     const int head = kv_head * p.group + row % p.group;
                     reinterpret_cast<uint2*>(p.output + ((static_cast<size_t>(entry) * p.tokens + token) * p.heads + head) * HEAD)[lane] =
                         make_uint2(pack_bf16x2(value[k].x, value[k].y), pack_bf16x2(value[k].z, value[k].w));
@@ -506,23 +459,31 @@ __global__ void __launch_bounds__(THREADS, 1) cross_forward_kernel(const __grid_
     }
 }
 
-// How a call's rows and keys are dealt to CTAs.
-constexpr double TILE_US = 1.75;            // a key tile in a CTA with one query tile
 
-struct Plan {
-    int cta_tiles, row_ctas, parts;
-};
+// Microseconds of a key tile in a CTA that has an SM to itself and in one of two that share it, and what a cluster costs beside its tiles (more when two of them
+// share their SMs): 3000 keys under 160 rows 44.2 us whole, 29.4, 22.3, 16.5, 13.9 in 2, 4, 6, 8 parts; 637 keys 10.2 whole, 11.3 in 5.
+constexpr double TILE_US = 1.7;
+constexpr double PAIR_US = 2.36;
+constexpr double JOIN_US = 7.0;
+constexpr double PAIR_JOIN_US = 10.0;
 
-Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
-    const int tile_tokens = TILE / (heads / kv_heads);
-    const long long row_tiles = (queries + tile_tokens - 1LL) / tile_tokens;
-    const long long pairs = static_cast<long long>(batch) * kv_heads;
-    Plan plan{};
-    plan.cta_tiles = row_tiles * pairs <= SMS ? 1 : 2;
-    plan.row_ctas = static_cast<int>((row_tiles + plan.cta_tiles - 1) / plan.cta_tiles);
-    // (with two tiles to a CTA there is one for every second SM already)
-    plan.parts = plan.cta_tiles == 1 ? loop_parts(plan.row_ctas * pairs, (keys + TILE - 1LL) / TILE, TILE_US, 8) : 1;
-    return plan;
+// Parts that the loop over `tiles` key tiles is cut into for `ctas` query tiles.
+int key_parts(long long ctas, long long tiles) {
+    const long long rest = ctas % (2 * SMS);
+    double best_us = static_cast<double>(tiles) * (static_cast<double>(ctas / (2 * SMS)) * PAIR_US + (rest == 0 ? 0.0 : rest <= SMS ? TILE_US : PAIR_US));
+    int best = 1;
+    for (int parts = 2; parts <= 8 && parts <= tiles; ++parts) {
+        if (ctas > 2LL * ACTIVE_CLUSTERS[parts]) {
+            break;
+        }
+        const bool alone = ctas <= ACTIVE_CLUSTERS[parts];
+        const double us = static_cast<double>((tiles + parts - 1) / parts) * (alone ? TILE_US : PAIR_US) + (alone ? JOIN_US : PAIR_JOIN_US);
+        if (us < best_us) {
+            best = parts;
+            best_us = us;
+        }
+    }
+    return best;
 }
 
 void configure() {
@@ -625,12 +586,12 @@ void flash_cross_forward_cuda(__nv_bfloat16* output, float* logsumexp, const __n
     p.group = group;
     p.scale = scale;
     p.scale_log2 = scale * LOG2E;
-    const Plan plan = make_plan(batch_size, query_length, key_length, query_heads, key_value_heads);
     p.output = output;
-    p.cta_tiles = plan.cta_tiles;
-    p.parts = plan.parts;
+    const long long row_tiles = (query_length + p.tile_tokens - 1LL) / p.tile_tokens;
+    p.parts = key_parts(row_tiles * key_value_heads * batch_size, (key_length + TILE - 1LL) / TILE);
     configure();
-    launch_chained_clusters(cross_forward_kernel, dim3(plan.row_ctas * plan.parts, key_value_heads, batch_size), plan.parts, dim3(THREADS), SMEM_BYTES, stream, p);
+    launch_chained_clusters(cross_forward_kernel, dim3(static_cast<unsigned>(row_tiles) * p.parts, key_value_heads, batch_size), p.parts, dim3(THREADS), SMEM_BYTES,
+                            stream, p);
 }
 
 }  // namespace dscuda
