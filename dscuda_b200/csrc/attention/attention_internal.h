@@ -52,6 +52,7 @@ int flash_decode_device_status(bool reset);
 int cross_forward_device_status(bool reset);
 int cross_backward_device_status(bool reset);
 int cross_backward_short_device_status(bool reset);
+int cross_query_short_device_status(bool reset);
 
 }  // namespace internal
 }  // namespace dscuda

@@ -13,6 +13,7 @@
 //   2. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
 //      key (two, half the rows each), P^T and dS^T back into tensor memory as bf16 A operands, dV += P^T dO, dK += dS^T Q.  Tensor memory: dV 128, dK
 //      128, two pairs of 64-column scores, so the scores of the next tile are computed while the softmax works on this one.
+// Short loops over many tiles take the forms of cross_query_short.cu and cross_backward_short.cu.
 // Where a grid of whole loops would leave SMs idle the loops are cut into parts for the CTAs of a cluster, which add their fp32 sums in order through
 // distributed shared memory (loop_parts.cuh).
 // S and dP are computed twice (1792 instead of 1280 FLOP per pair).  The alternative of the causal backward, dS stored once and streamed
@@ -849,7 +850,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
 
 struct Plan {
     int query_parts, key_parts;
-    bool key_short;
+    bool query_short, key_short;
 };
 
 Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
@@ -859,7 +860,8 @@ Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
     const long long sub_tiles = (queries + SUB / group - 1LL) / (SUB / group);
     const long long pairs = static_cast<long long>(batch) * kv_heads;
     const int key_parts = loop_parts(key_tiles * pairs, sub_tiles, KEY_TILE_US, MOST_KEY_PARTS);
-    return {loop_parts(row_tiles * pairs, key_tiles, QUERY_TILE_US, 8), key_parts, key_parts == 1 && cross_key_short_takes(key_tiles * pairs, sub_tiles)};
+    const int query_parts = loop_parts(row_tiles * pairs, key_tiles, QUERY_TILE_US, 8);
+    return {query_parts, key_parts, query_parts == 1 && cross_query_short_takes(row_tiles * pairs, key_tiles), key_parts == 1 && cross_key_short_takes(key_tiles * pairs, sub_tiles)};
 }
 
 void configure() {
@@ -949,8 +951,12 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     p.batch = batch_size;
     p.key_tiles = (key_length + BIG - 1) / BIG;
     configure();
-    launch_chained_clusters(cross_query_kernel, dim3((query_length + p.big_tokens - 1) / p.big_tokens * plan.query_parts, key_value_heads, batch_size),
-                            plan.query_parts, dim3(THREADS), queryside::SMEM_BYTES, stream, p);
+    if (plan.query_short) {
+        launch_cross_query_short(p, stream);
+    } else {
+        launch_chained_clusters(cross_query_kernel, dim3((query_length + p.big_tokens - 1) / p.big_tokens * plan.query_parts, key_value_heads, batch_size),
+                                plan.query_parts, dim3(THREADS), queryside::SMEM_BYTES, stream, p);
+    }
     if (plan.key_short) {
         launch_cross_key_short(p, stream);
         return;

@@ -1,4 +1,4 @@
-// What the two files of the cross attention's gradients share: sizes, parameters, output staging.
+// What the files of the cross attention's gradients share: sizes, parameters, output staging.
 #pragma once
 
 #include "sm100_primitives.cuh"
@@ -63,5 +63,9 @@ __device__ __forceinline__ void stage_bf16x32(uint8_t* chunk, int r, int half, c
 // The key kernel for short loops (cross_backward_short.cu): whether it takes a call with that many items of 128 keys and row tiles, and its launch.
 bool cross_key_short_takes(long long items, long long row_tiles);
 void launch_cross_key_short(const cross::CrossBackwardParams& p, cudaStream_t stream);
+
+// The same for the query kernel (cross_query_short.cu), items of 128 rows.
+bool cross_query_short_takes(long long items, long long key_tiles);
+void launch_cross_query_short(const cross::CrossBackwardParams& p, cudaStream_t stream);
 
 }  // namespace dscuda

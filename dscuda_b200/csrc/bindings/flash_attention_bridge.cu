@@ -115,7 +115,7 @@ extern "C" int dscuda_flash_device_status(int reset) {
         // every word is read (and reset); the first that is not 0 is reported
         int status = 0;
         for (int (*word)(bool) : {forward_device_status, flash_cache_device_status, flash_decode_device_status, cross_forward_device_status,
-                                  cross_backward_device_status, cross_backward_short_device_status}) {
+                                  cross_backward_device_status, cross_backward_short_device_status, cross_query_short_device_status}) {
             const int value = word(reset != 0);
             status = status != 0 ? status : value;
         }

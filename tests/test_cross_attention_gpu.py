@@ -62,6 +62,11 @@ SHAPES += [
     (40, 5, 700, 8, 4, [(97 * i) % 701 for i in range(40)]), (2, 12, 5000, 28, 4, [5000, 2500]), (1, 700, 4850, 8, 8, None), (70, 3, 130, 6, 3, [0, 130, 128, 1, 129] * 14),
     (5, 90, 1100, 12, 12, [0, 0, 0, 0, 1]),
 ]
+# few keys under many rows: CTAs of the query kernel that go over several items
+SHAPES += [
+    (6, 900, 300, 16, 8, [300, 0, 128, 129, 1, 257]), (3, 4000, 20, 8, 4, [20, 3, 17]), (2, 3000, 1000, 14, 2, [1000, 129]), (40, 130, 500, 8, 8, [(53 * i) % 501 for i in range(40)]),
+    (1, 5000, 700, 24, 8, None), (2, 2400, 64, 8, 8, None), (3, 1700, 256, 33, 11, [0, 256, 100]),
+]
 
 
 @pytest.mark.parametrize("b,tq,tk,hq,hkv,lengths", SHAPES)
@@ -71,7 +76,7 @@ def test_forward_and_gradients(gpu, b, tq, tk, hq, hkv, lengths):
 
 
 @pytest.mark.parametrize("b,tq,tk,hq,hkv,lengths", [(2, 1, 300, 8, 2, [290, 7]), (3, 77, 333, 6, 2, [300, 0, 128]), (2, 200, 1000, 8, 1, [999, 1]),
-                                                      (2, 20, 2600, 8, 2, [2500, 130]), (40, 5, 700, 8, 4, [(97 * i) % 701 for i in range(40)])])
+                                                      (2, 20, 2600, 8, 2, [2500, 130]), (40, 5, 700, 8, 4, [(97 * i) % 701 for i in range(40)]), (6, 900, 300, 16, 8, [290, 0, 128, 129, 1, 257])])
 def test_padding_is_never_used(gpu, b, tq, tk, hq, hkv, lengths):
     """NaN or infinities behind the lengths: the same bits as zeros there."""
     query, key, value, dout = inputs(gpu, b, tq, tk, hq, hkv)
