@@ -15,7 +15,7 @@
 // tokens and short drafts are what this is for, so the one form serves all.
 //
 // Measured (64 query heads on 8): 32 sequences of 1000-8000 tokens 46.5 us (floor 38.3), 4 drafted tokens at 20000-40000 120 us (floor
-// 72.7; bound by the issue of widening and softmax beside the copies), one sequence of 100 tokens 8.3 us (two launches).
+// 72.7; bound by the issue of widening and softmax beside the copies), one sequence of 100 tokens 4.0 us (one launch; 5.4 in parts).
 //
 // Operands.  Codes become f16 (exact for both types: int8 through 1024 + u - 1152, e4m3 by conversion) and so does Q, each row
 // multiplied by a power of two that brings its largest element to 2^13..2^14; P is rounded to f16 (half a step is 2^-11 of it), relative to the
@@ -31,8 +31,8 @@
 //
 // Work split: tiles of 4 warps x 32 (16) keys of all (sequence, head, row block) items laid end to end and cut into equal ranges, one
 // per CTA.  A warp streams its own keys through its own ring (cp.async, no barriers between warps); the four merge at the end of an
-// item.  An item that one CTA sees whole is written at once, parts go to the workspace, and the CTA with an item's first tile leaves a
-// note of who holds them; flash_decode_combine_kernel joins them.  No atomics: results do not depend on the order in which CTAs run.
+// item.  Short items stay whole (stays_whole).  Otherwise an item that one CTA sees whole is written at once, parts go to the workspace, and the CTA with an item's first tile leaves a
+// note of who holds them; flash_decode_combine_kernel joins them.  Where all items are short each stays with a CTA of its own (stays_whole).  No atomics: results do not depend on the order in which CTAs run.
 #include "flash_attention.h"
 #include "cuda_common.h"
 #include "attention_internal.h"
@@ -91,6 +91,7 @@ struct DecodeParams {
     int keys_most;                      // pages * page, or Tk
     int row_blocks;
     int causal;                         // token t sees keys < length - tokens + 1 + t
+    int whole;                          // a CTA to an item, no parts
     float scale;
 };
 
@@ -207,11 +208,27 @@ __device__ __forceinline__ size_t lse_offset(const DecodeParams& p, int b, int k
 
 // Equal ranges of tiles: the first total % ctas CTAs take one more than the others.
 struct Ranges {
-    unsigned each, more;
+    unsigned each = 0, more = 0;
+    Ranges() = default;
     __device__ Ranges(unsigned total, unsigned ctas) : each(total / ctas), more(total % ctas) {}
     __device__ unsigned start(unsigned cta) const { return each * cta + min(cta, more); }
     __device__ unsigned holder(unsigned tile) const { return tile < (each + 1) * more ? tile / (each + 1) : more + (tile - (each + 1) * more) / each; }
 };
+
+// An item of an entry without keys: zeros and -inf.
+template <int ROWS>
+__device__ void write_empty_rows(const DecodeParams& p, int entry, int item) {
+    const int kv_head = item / p.row_blocks;
+    const int row_base = (item - kv_head * p.row_blocks) * ROWS;
+    const int rows = min(ROWS, p.group * p.tokens - row_base);
+    for (int unit = threadIdx.x; unit < rows * (HEAD / 8); unit += THREADS) {
+        const int row = row_base + unit / (HEAD / 8);
+        reinterpret_cast<uint4*>(p.out + row_offset(p, entry, kv_head, row))[unit % (HEAD / 8)] = make_uint4(0, 0, 0, 0);
+        if (unit % (HEAD / 8) == 0) {
+            p.lse[lse_offset(p, entry, kv_head, row)] = -INFINITY;
+        }
+    }
+}
 
 template <int SOURCE, int NB>
 __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash_decode_kernel(const __grid_constant__ DecodeParams p) {
@@ -245,38 +262,51 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
     sm100::grid_dependency_wait();
     // ---- the CTA's range of tiles, and the entry that holds its first one; every warp for itself --------------
     const unsigned items = p.kv_heads * p.row_blocks;
-    unsigned total = 0, own = 0;
-    for (int base = 0; base < p.batch; base += 32) {
-        own = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
-        total += __reduce_add_sync(0xffffffffU, own);
-    }
-    const unsigned ctas = min(total, gridDim.x);
-    if (blockIdx.x >= ctas) {
-        return;
-    }
-    const Ranges ranges(total, ctas);
-    unsigned position = ranges.start(blockIdx.x);
-    const unsigned end = ranges.start(blockIdx.x + 1);
-    unsigned entry_first = 0;
+    Ranges ranges;
+    unsigned position, end, entry_first = 0;
     int entry = 0;
-    for (int base = 0;; base += 32) {
-        if (p.batch > 32) {
+    if (p.whole != 0) {
+        entry = static_cast<int>(blockIdx.x / items);
+        const unsigned item = blockIdx.x - entry * items;
+        const int length = length_of(p, entry);
+        if (length == 0) {
+            write_empty_rows<S::ROWS>(p, entry, static_cast<int>(item));
+            return;
+        }
+        position = item * item_cost(length, S::TILE);
+        end = position + item_cost(length, S::TILE);
+    } else {
+        unsigned total = 0, own = 0;
+        for (int base = 0; base < p.batch; base += 32) {
             own = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
+            total += __reduce_add_sync(0xffffffffU, own);
         }
-        unsigned inclusive = own;
+        const unsigned ctas = min(total, gridDim.x);
+        if (blockIdx.x >= ctas) {
+            return;
+        }
+        ranges = Ranges(total, ctas);
+        position = ranges.start(blockIdx.x);
+        end = ranges.start(blockIdx.x + 1);
+        for (int base = 0;; base += 32) {
+            if (p.batch > 32) {
+                own = base + lane < p.batch ? item_cost(length_of(p, base + lane), S::TILE) * items : 0;
+            }
+            unsigned inclusive = own;
 #pragma unroll
-        for (int offset = 1; offset < 32; offset <<= 1) {
-            const unsigned other = __shfl_up_sync(0xffffffffU, inclusive, offset);
-            inclusive += lane >= offset ? other : 0;
+            for (int offset = 1; offset < 32; offset <<= 1) {
+                const unsigned other = __shfl_up_sync(0xffffffffU, inclusive, offset);
+                inclusive += lane >= offset ? other : 0;
+            }
+            const unsigned mine = __ballot_sync(0xffffffffU, position < entry_first + inclusive);
+            if (mine != 0) {
+                const int source = __ffs(mine) - 1;
+                entry = base + source;
+                entry_first += __shfl_sync(0xffffffffU, inclusive - own, source);
+                break;
+            }
+            entry_first += __shfl_sync(0xffffffffU, inclusive, 31);
         }
-        const unsigned mine = __ballot_sync(0xffffffffU, position < entry_first + inclusive);
-        if (mine != 0) {
-            const int source = __ffs(mine) - 1;
-            entry = base + source;
-            entry_first += __shfl_sync(0xffffffffU, inclusive - own, source);
-            break;
-        }
-        entry_first += __shfl_sync(0xffffffffU, inclusive, 31);
     }
 
     bool first_segment = true;
@@ -702,7 +732,7 @@ __global__ void __launch_bounds__(THREADS, Shape<SOURCE, NB>::CTAS_PER_SM) flash
         __syncthreads();
         const bool whole = tile_begin == 0 && tile_end == entry_tiles;
         const unsigned slot = 2 * blockIdx.x + (first_segment ? 0 : 1);
-        if (tile_begin == 0 && threadIdx.x == 0) {
+        if (tile_begin == 0 && threadIdx.x == 0 && p.whole == 0) {
             const int holders = static_cast<int>(ranges.holder(first_tile + entry_tiles - 1) - blockIdx.x) + 1;
             p.notes[static_cast<size_t>(entry) * items + item] = {static_cast<int>(blockIdx.x), 2 * holders + (first_segment ? 0 : 1)};
         }
@@ -867,6 +897,14 @@ __global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __g
     }
 }
 
+// Whether every item stays whole, with a CTA of its own and no second kernel: up to so many keys the time of the longest item is below that of the parts and
+// their joining.  us, parts and whole: 8 items of 250 keys 6.4 and 4.9, 380 6.4 and 5.7, 500 6.5 and 6.6; 128 items of 100 keys 7.3 and 4.3, 500 10.1 and 6.9,
+// 1000 11.6 and 10.1; 512 items of 500 17.3 and 15.2, 1000 28.3 and 33.5; bf16 states 128 items of 100 keys 6.6 and 3.7, 512 of 500 27.1 and 26.2.  (The longest
+// is what the caller's table or tensor holds; lengths are not known here.)
+bool stays_whole(long long items, int keys_most, int at_once) {
+    return keys_most <= (items > at_once ? 512 : items >= 96 ? 1024 : items >= 32 ? 640 : 384);
+}
+
 // Rows up to which each has a CTA of the joining kernel.  Both kernels with a warp and a CTA to a row: 8 rows over 40000 keys 52.3 and 15.8 us, 128 over
 // 3000 12.6 and 10.2, 1024 over 5000 21.8 and 22.1, 2048 over 600 14.8 and 16.8.
 constexpr long long WIDE_COMBINE_ROWS = 512;
@@ -897,6 +935,12 @@ void launch_decode(DecodeParams& p, cudaStream_t stream) {
         if (device < 16) {
             done[device] = true;
         }
+    }
+    const long long items = static_cast<long long>(p.batch) * p.kv_heads * p.row_blocks;
+    p.whole = stays_whole(items, p.keys_most, 148 * S::CTAS_PER_SM);
+    if (p.whole != 0) {
+        launch_chained(flash_decode_kernel<SOURCE, NB>, dim3(static_cast<unsigned>(items)), dim3(THREADS), S::BYTES, stream, p);
+        return;
     }
     const int ctas = static_cast<int>(std::min<long long>(148LL * S::CTAS_PER_SM, most));
     p.part_lse = p.part_out + static_cast<size_t>(2 * MOST_CTAS) * S::ROWS * HEAD;

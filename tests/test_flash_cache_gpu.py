@@ -169,6 +169,16 @@ def test_decode_long_and_many(gpu):
     decode_and_compare(gpu, torch.int8, [30000, 0, 70, 15000], 8, 8, 2, 64, 35)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("lengths,tokens,hq,hkv,page", [
+    # on both sides of the change from whole items to parts (it depends on the keys that a table holds and the number of items)
+    ([384, 0], 1, 8, 2, 64), ([400, 0], 1, 8, 2, 16), ([1024 - 7 * i for i in range(48)], 1, 8, 2, 64), ([1040, 0, 3] * 16, 1, 8, 2, 16),
+    ([0] * 3 + [512, 500] * 90, 2, 15, 3, 32), ([528, 1, 0] * 60, 1, 12, 3, 16), ([0, 0, 1] * 40, 8, 32, 4, 32), ([0, 100], 64, 6, 1, 32), ([0, 0], 3, 4, 4, 16),
+])
+def test_whole_items_and_parts(gpu, kind, lengths, tokens, hq, hkv, page):
+    decode_and_compare(gpu, kind, lengths, tokens, hq, hkv, page, 60)
+
+
 def test_lengths_behind_the_table_and_large_queries(gpu):
     decode_and_compare(gpu, torch.int8, [1000, -3], 1, 8, 2, 64, 34, pages=3)
     # sharp softmax, values of Q far from 1 on both sides: the power of two in front of f16
