@@ -57,7 +57,7 @@ namespace keyside {
 constexpr int STAGES = 4;
 constexpr int STAGE_BYTES = 4 * SUB_CHUNK;          // Q and dO of 64 rows
 constexpr int RESIDENT_BYTES = 4 * BIG_CHUNK;       // K and V of 128 keys
-constexpr int MISC_BYTES = 3072;
+constexpr int MISC_BYTES = 2560;
 constexpr int SMEM_BYTES = RESIDENT_BYTES + STAGES * STAGE_BYTES + MISC_BYTES + 1024;
 constexpr uint32_t TMEM_DV = 0;
 constexpr uint32_t TMEM_DK = 128;
@@ -409,7 +409,7 @@ constexpr int Q_BYTES = 2 * BIG_CHUNK;
 constexpr int TILE_BYTES = 2 * BIG_CHUNK;
 constexpr int K_SLOTS = 3;
 constexpr int V_SLOTS = 2;
-constexpr int MISC_BYTES = 3072;
+constexpr int MISC_BYTES = 2560;
 constexpr int SMEM_BYTES = Q_BYTES + (K_SLOTS + V_SLOTS) * TILE_BYTES + MISC_BYTES + 1024;
 constexpr uint32_t TMEM_S = 0;
 constexpr uint32_t TMEM_DP = 128;

@@ -10,7 +10,6 @@
 #include "loop_parts.cuh"
 #include "../common/launch.h"
 
-#include <algorithm>
 #include <cstdint>
 
 namespace dscuda {

@@ -17,7 +17,8 @@ constexpr long long SMS = 148;
 // the groups of 16 to 20 SMs that share a network).  One more waits for a whole wave: 16 clusters of 8 took 42 us where 15 of 7 take 27.
 constexpr int ACTIVE_CLUSTERS[17] = {0, 148, 74, 45, 33, 26, 22, 15, 15, 0, 0, 0, 0, 0, 0, 0, 7};
 
-// What a cluster costs beside its loops: launch, two cluster barriers, the reads.  40 heads' rows over 4 key tiles: 11.2 us whole, 11.4 in four parts.
+// What a cluster costs beside its loops in the gradients' kernels: launch, two cluster barriers, the reads.  (Backward of 4064 x 3 rows over 3 x 3821 ragged keys, 180
+// whole loops for 148 SMs: 233 us whole, 144 in parts.)
 constexpr double CLUSTER_US = 4.3;
 
 // Parts that a loop of `tiles` tiles of `tile_us` microseconds is cut into when `ctas` whole loops would run: the cluster size (up to `most`: 8 is portable, 16 has
