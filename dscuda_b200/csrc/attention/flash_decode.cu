@@ -898,11 +898,11 @@ __global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __g
 }
 
 // Whether every item stays whole, with a CTA of its own and no second kernel: up to so many keys the time of the longest item is below that of the parts and
-// their joining.  us, parts and whole: 8 items of 250 keys 6.4 and 4.9, 380 6.4 and 5.7, 500 6.5 and 6.6; 128 items of 100 keys 7.3 and 4.3, 500 10.1 and 6.9,
-// 1000 11.6 and 10.1; 512 items of 500 17.3 and 15.2, 1000 28.3 and 33.5; bf16 states 128 items of 100 keys 6.6 and 3.7, 512 of 500 27.1 and 26.2.  (The longest
-// is what the caller's table or tensor holds; lengths are not known here.)
+// their joining.  us, parts and whole, lengths down to a third or less: 32 items of up to 400 keys 9.4 and 6.8, 640 8.7 and 8.0; 64 of 900 10.3 and 10.4; 128 of 512
+// 10.8 and 8.2, 768 12.5 and 10.0, bf16 states of 1000 13.0 and 13.6; 200 of 1000 15.0 and 14.0, 1500 16.6 and 16.4, 2000 18.3 and 21.4; 512 of 512 17.8 and 15.7, 800
+// 19.6 and 19.3, 1200 25.6 and 27.1.  (The longest is what the caller's table or tensor holds; lengths are not known here.)
 bool stays_whole(long long items, int keys_most, int at_once) {
-    return keys_most <= (items > at_once ? 512 : items >= 96 ? 1024 : items >= 32 ? 640 : 384);
+    return keys_most <= (items > at_once ? 768 : items >= 200 ? 1280 : items >= 96 ? 896 : items >= 32 ? 704 : 384);
 }
 
 // Rows up to which each has a CTA of the joining kernel.  Both kernels with a warp and a CTA to a row: 8 rows over 40000 keys 52.3 and 15.8 us, 128 over
