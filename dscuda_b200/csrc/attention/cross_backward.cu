@@ -9,7 +9,8 @@
 //   1. cross_query_kernel: a CTA keeps 128 rows (Q, dO) and goes over the keys in tiles of 128: S = Q K^T, dP = dO V^T, dQ += dS K.  It forms delta from the
 //      O rows first, and leaves lse * log2(e) and delta in row order for the next kernel.  With few keys the rounding of O in delta would be the largest error
 //      of dS (2 keys: 0.4 % of dQ and dK, against 0.17 % of the last rounding); where one tile holds all keys, delta = sum_k P dP is formed
-//      from the tile itself.
+//      from the tile itself.  One key has no gradient at all (its weight is 1 whatever the score): dS is set to zero on both sides, where dP - delta would
+//      leave what two orders of the same sum differ by.
 //   2. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
 //      key (two, half the rows each), P^T and dS^T back into tensor memory as bf16 A operands, dV += P^T dO, dK += dS^T Q.  Tensor memory: dV 128, dK
 //      128, two pairs of 64-column scores, so the scores of the next tile are computed while the softmax works on this one.
@@ -268,6 +269,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
         const int group = warp / 4;
         const int r = threadIdx.x % BIG;
         const uint32_t lane_base = static_cast<uint32_t>((warp % 4) * 32) << 16;
+        const float ds_scale = length == 1 ? 0.0F : p.scale;       // (the weight of a single key is 1 whatever the score)
         bool alive = true;
         for (int t = 0; t < tile_count; ++t) {
             const int stage = t % STAGES;
@@ -311,9 +313,9 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_kernel(const __grid_cons
 #pragma unroll
             for (int n = 0; n < 32; n += 4) {
                 const float4 d = delta4[n / 4];
-                packed[n / 2] = pack_bf16x2(prob[n] * (__uint_as_float(sb[n]) - d.x) * p.scale, prob[n + 1] * (__uint_as_float(sb[n + 1]) - d.y) * p.scale);
+                packed[n / 2] = pack_bf16x2(prob[n] * (__uint_as_float(sb[n]) - d.x) * ds_scale, prob[n + 1] * (__uint_as_float(sb[n + 1]) - d.y) * ds_scale);
                 packed[n / 2 + 1] =
-                    pack_bf16x2(prob[n + 2] * (__uint_as_float(sb[n + 2]) - d.z) * p.scale, prob[n + 3] * (__uint_as_float(sb[n + 3]) - d.w) * p.scale);
+                    pack_bf16x2(prob[n + 2] * (__uint_as_float(sb[n + 2]) - d.z) * ds_scale, prob[n + 3] * (__uint_as_float(sb[n + 3]) - d.w) * ds_scale);
             }
             tmem_st_x16(s_tmem + 64, packed);
             tmem_wait_st();
@@ -733,7 +735,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                 prob[n] = exp2_approx(fmaf(__uint_as_float(sb[n]), p.scale_log2, -lse2)) * p.scale;
             }
             if (j + 1 == tile_count) {
-                const int present = left - j * KEYS - half * 64;
+                // (a single key's weight is 1 whatever the score: none counts here)
+                const int present = length == 1 ? 0 : left - j * KEYS - half * 64;
 #pragma unroll
                 for (int n = 0; n < 64; ++n) {
                     prob[n] = n < present ? prob[n] : 0.0F;

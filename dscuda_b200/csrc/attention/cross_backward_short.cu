@@ -393,7 +393,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_key_short_kernel(const __gri
                     break;
                 }
                 tc_fence_after_sync();
-                score_gradients(prob, s_tmem + 64, bars->delta[stage] + group * 32, p.scale);
+                score_gradients(prob, s_tmem + 64, bars->delta[stage] + group * 32, at.length == 1 ? 0.0F : p.scale);      // (one key: its weight is 1 whatever the score)
                 tc_fence_before_sync();
                 mbar_arrive(smem_u32(&bars->ds_full[t & 1]));
             }

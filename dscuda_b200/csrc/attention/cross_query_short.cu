@@ -395,7 +395,8 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_short_kernel(const __g
                     prob[k] = exp2_approx(fmaf(__uint_as_float(sb[k]), p.scale_log2, -lse2)) * p.scale;
                 }
                 if (j + 1 == tile_count) {
-                    const int present = at.length - j * KEYS - half * 64;
+                    // (a single key's weight is 1 whatever the score: none counts here)
+                    const int present = at.length == 1 ? 0 : at.length - j * KEYS - half * 64;
 #pragma unroll
                     for (int k = 0; k < 64; ++k) {
                         prob[k] = k < present ? prob[k] : 0.0F;
