@@ -140,3 +140,73 @@ def cross_gradients(dout, query, key, value, scale, lengths):
             slacks[2][b, :n, g] += p_err.t() @ do.abs()
     # fp32 sums over rows and keys, and the last rounding
     return grads, [(1 + BF16) * s * (1 + 2.0 ** -10) + BF16 * g.abs() + 2.0 ** -40 for s, g in zip(slacks, grads)]
+
+
+# ---- the same errors added as independent ones --------------------------------------------------------------------------
+# The bounds above hold for any signs of the roundings and so grow with the number of terms, where the errors of a long sum grow with its root: a
+# missing tile of a long loop stays below them.  A rounding's error is spread over +-half a step, at most `step` times the value, so
+# its variance is at most (step value)^2 / 3; the sum of squared errors of a head's result is near the sum of their variances.
+
+EXACT_DELTA = 128               # up to so many keys the gradients' delta is formed from P and dP, not from the rounded output
+
+
+def _variance(values, step):
+    return (step * values) ** 2 / 3
+
+
+def attention_variances(query, keys, values, scale, limits, weight_step):
+    """Output of `attention` [T, Hq, 128] and the variance of each element."""
+    t, hq, _ = query.shape
+    if not keys.shape[0]:
+        return (torch.zeros(t, hq, 128, dtype=torch.float64, device=query.device),) * 2
+    group = hq // keys.shape[1]
+    out, variance = (torch.empty(t, hq, 128, dtype=torch.float64, device=query.device) for _ in range(2))
+    seen = torch.arange(keys.shape[0], device=query.device)[None] < limits.to(query.device)[:, None]
+    for h in range(hq):
+        q, k, v = query[:, h].double(), keys[:, h // group].double(), values[:, h // group].double()
+        scores = torch.where(seen, q @ k.t() * scale, -math.inf)
+        p = torch.nan_to_num(torch.softmax(scores, -1))                                  # (zeros where nothing is seen)
+        e = EXP + 2 * SUM * torch.where(seen, q.abs() @ k.abs().t() * scale, 0.0).amax(-1, keepdim=True)
+        out[:, h] = p @ v
+        tiny = keys.shape[0] * (2.0 ** -32 * v.abs().amax()) ** 2                         # weights far below the largest one in f16
+        variance[:, h] = _variance(out[:, h], BF16) + (weight_step ** 2 / 3 + e ** 2) * (p ** 2 @ v ** 2) + (e * out[:, h]) ** 2 + tiny
+    return out, variance
+
+
+def cross_variances(dout, query, key, value, scale, lengths, exact_delta=EXACT_DELTA):
+    """output, dquery, dkey, dvalue and the variance of each of their elements."""
+    shapes = (query, query, key, value)
+    results, variances = ([torch.zeros(x.shape, dtype=torch.float64, device=x.device) for x in shapes] for _ in range(2))
+    group = query.shape[2] // key.shape[2]
+    for b, n in enumerate(lengths):
+        for h in range(query.shape[2] if n else 0):
+            g = h // group
+            q, k, v, do = query[b, :, h].double(), key[b, :n, g].double(), value[b, :n, g].double(), dout[b, :, h].double()
+            p = torch.softmax(q @ k.t() * scale, -1)
+            e = EXP + 3 * SUM * (q.abs() @ k.abs().t() * scale).amax(-1, keepdim=True)     # relative error of P
+            weights = (BF16 ** 2 / 3 + e ** 2) * p ** 2
+            out, dp = p @ v, do @ v.t()
+            out_variance = _variance(out, BF16) + weights @ v ** 2
+            delta = (do * out).sum(-1, keepdim=True)
+            delta_variance = (e * delta) ** 2 + (SUM * (do * out).abs().sum(-1, keepdim=True)) ** 2
+            if n > exact_delta:
+                delta_variance = delta_variance + (do ** 2 * out_variance).sum(-1, keepdim=True)
+            ds = p * (dp - delta) * scale
+            ds_variance = (BF16 ** 2 / 3 + e ** 2) * ds ** 2 + (p * scale * SUM * (do.abs() @ v.abs().t())) ** 2
+            shared = delta_variance * scale ** 2                                          # one error of delta for all of a row
+            results[0][b, :, h], variances[0][b, :, h] = out, out_variance
+            results[1][b, :, h] = ds @ k
+            variances[1][b, :, h] = ds_variance @ k ** 2 + shared * (p @ k) ** 2 + (e * (ds @ k)) ** 2
+            results[2][b, :n, g] += ds.t() @ q
+            variances[2][b, :n, g] += ds_variance.t() @ q ** 2 + (shared * p ** 2).t() @ q ** 2
+            results[3][b, :n, g] += p.t() @ do
+            variances[3][b, :n, g] += weights.t() @ do ** 2
+    for x, variance in zip(results[1:], variances[1:]):
+        variance += _variance(x, BF16)
+    return results, variances
+
+
+def deviations(actual, expected, variance):
+    """How many times the root of its summed variances the error of a head is, the largest over entries and heads of [B, T, H, 128]."""
+    error, allowed = ((actual.double() - expected) ** 2).sum((1, 3)), variance.sum((1, 3))
+    return float(torch.where(error > 0, (error / allowed).sqrt(), torch.zeros_like(error)).max())
