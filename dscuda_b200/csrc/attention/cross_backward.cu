@@ -851,35 +851,35 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
     }
 }
 
+struct Clusters {
+    ClusterCounts query, key;
+};
+
 struct Plan {
     int query_parts, key_parts;
     bool query_short, key_short;
 };
 
-Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads) {
+Plan make_plan(int batch, int queries, int keys, int heads, int kv_heads, const Clusters& clusters) {
     const int group = heads / kv_heads;
     const long long key_tiles = (keys + BIG - 1LL) / BIG;
     const long long row_tiles = (queries + BIG / group - 1LL) / (BIG / group);
     const long long sub_tiles = (queries + SUB / group - 1LL) / (SUB / group);
     const long long pairs = static_cast<long long>(batch) * kv_heads;
-    const int key_parts = loop_parts(key_tiles * pairs, sub_tiles, KEY_TILE_US, MOST_KEY_PARTS);
-    const int query_parts = loop_parts(row_tiles * pairs, key_tiles, QUERY_TILE_US, 8);
+    const int key_parts = loop_parts(key_tiles * pairs, sub_tiles, KEY_TILE_US, clusters.key);
+    const int query_parts = loop_parts(row_tiles * pairs, key_tiles, QUERY_TILE_US, clusters.query);
     return {query_parts, key_parts, query_parts == 1 && cross_query_short_takes(row_tiles * pairs, key_tiles), key_parts == 1 && cross_key_short_takes(key_tiles * pairs, sub_tiles)};
 }
 
-void configure() {
-    static bool done[16] = {};
-    int device = 0;
-    CUDA_CHECK(cudaGetDevice(&device));
-    if (device < 16 && done[device]) {
-        return;
-    }
-    CUDA_CHECK(cudaFuncSetAttribute(cross_key_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, keyside::SMEM_BYTES));
-    CUDA_CHECK(cudaFuncSetAttribute(cross_key_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
-    CUDA_CHECK(cudaFuncSetAttribute(cross_query_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, queryside::SMEM_BYTES));
-    if (device < 16) {
-        done[device] = true;
-    }
+const Clusters& configure() {
+    static PerDevice<Clusters> devices;
+    return devices.get([] {
+        CUDA_CHECK(cudaFuncSetAttribute(cross_key_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, keyside::SMEM_BYTES));
+        CUDA_CHECK(cudaFuncSetAttribute(cross_key_kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+        CUDA_CHECK(cudaFuncSetAttribute(cross_query_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, queryside::SMEM_BYTES));
+        return Clusters{cluster_counts(cross_query_kernel, THREADS, queryside::SMEM_BYTES, 8),
+                        cluster_counts(cross_key_kernel, THREADS, keyside::SMEM_BYTES, MOST_KEY_PARTS)};
+    });
 }
 
 }  // namespace
@@ -937,7 +937,7 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     if ((key_length + BIG - 1LL) / BIG * key_value_heads * batch_size > 0x7fffffffLL) {
         throw std::invalid_argument("flash cross attention shape exceeds the supported index range");
     }
-    const Plan plan = make_plan(batch_size, query_length, key_length, query_heads, key_value_heads);
+    const Plan plan = make_plan(batch_size, query_length, key_length, query_heads, key_value_heads, configure());
     p.rows = static_cast<float2*>(workspace);
     p.dq_out = query_gradient;
     p.dk_out = key_gradient;
@@ -953,7 +953,6 @@ void flash_cross_backward_cuda(__nv_bfloat16* query_gradient, __nv_bfloat16* key
     p.scale_log2 = scale * LOG2E;
     p.batch = batch_size;
     p.key_tiles = (key_length + BIG - 1) / BIG;
-    configure();
     if (plan.query_short) {
         launch_cross_query_short(p, stream);
     } else {

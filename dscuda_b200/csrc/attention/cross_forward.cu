@@ -468,15 +468,15 @@ constexpr double JOIN_US = 7.0;
 constexpr double PAIR_JOIN_US = 10.0;
 
 // Parts that the loop over `tiles` key tiles is cut into for `ctas` query tiles.
-int key_parts(long long ctas, long long tiles) {
+int key_parts(long long ctas, long long tiles, const ClusterCounts& counts) {
     const long long rest = ctas % (2 * SMS);
     double best_us = static_cast<double>(tiles) * (static_cast<double>(ctas / (2 * SMS)) * PAIR_US + (rest == 0 ? 0.0 : rest <= SMS ? TILE_US : PAIR_US));
     int best = 1;
     for (int parts = 2; parts <= 8 && parts <= tiles; ++parts) {
-        if (ctas > 2LL * ACTIVE_CLUSTERS[parts]) {
+        if (ctas > 2LL * counts.of[parts]) {            // (the device counts one CTA to an SM)
             break;
         }
-        const bool alone = ctas <= ACTIVE_CLUSTERS[parts];
+        const bool alone = ctas <= counts.of[parts];
         const double us = static_cast<double>((tiles + parts - 1) / parts) * (alone ? TILE_US : PAIR_US) + (alone ? JOIN_US : PAIR_JOIN_US);
         if (us < best_us) {
             best = parts;
@@ -486,17 +486,12 @@ int key_parts(long long ctas, long long tiles) {
     return best;
 }
 
-void configure() {
-    static bool done[16] = {};
-    int device = 0;
-    CUDA_CHECK(cudaGetDevice(&device));
-    if (device < 16 && done[device]) {
-        return;
-    }
-    CUDA_CHECK(cudaFuncSetAttribute(cross_forward_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
-    if (device < 16) {
-        done[device] = true;
-    }
+const ClusterCounts& configure() {
+    static PerDevice<ClusterCounts> devices;
+    return devices.get([] {
+        CUDA_CHECK(cudaFuncSetAttribute(cross_forward_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES));
+        return cluster_counts(cross_forward_kernel, THREADS, SMEM_BYTES, 8);
+    });
 }
 
 // Rows to a key head up to which flash_decode.cu's kernels take the call.
@@ -588,8 +583,7 @@ void flash_cross_forward_cuda(__nv_bfloat16* output, float* logsumexp, const __n
     p.scale_log2 = scale * LOG2E;
     p.output = output;
     const long long row_tiles = (query_length + p.tile_tokens - 1LL) / p.tile_tokens;
-    p.parts = key_parts(row_tiles * key_value_heads * batch_size, (key_length + TILE - 1LL) / TILE);
-    configure();
+    p.parts = key_parts(row_tiles * key_value_heads * batch_size, (key_length + TILE - 1LL) / TILE, configure());
     launch_chained_clusters(cross_forward_kernel, dim3(static_cast<unsigned>(row_tiles) * p.parts, key_value_heads, batch_size), p.parts, dim3(THREADS), SMEM_BYTES,
                             stream, p);
 }

@@ -8,29 +8,59 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <cstddef>
 #include <cstdint>
 
 namespace dscuda {
 
 constexpr long long SMS = 148;
-// Clusters of 1, 2 .. 8 and of 16 CTAs, one CTA to an SM, that a B200 holds at a time (cudaOccupancyMaxActiveClusters: a cluster stays inside one of
-// the groups of 16 to 20 SMs that share a network).  One more waits for a whole wave: 16 clusters of 8 took 42 us where 15 of 7 take 27.
-constexpr int ACTIVE_CLUSTERS[17] = {0, 148, 74, 45, 33, 26, 22, 15, 15, 0, 0, 0, 0, 0, 0, 0, 7};
+constexpr int MOST_PARTS = 16;
+
+// Clusters of n CTAs of a kernel that a device holds at a time, of[n]; 0 for sizes that it cannot launch (a cluster stays inside one of the groups of 16 to
+// 20 SMs that share a network, and these differ from one device or partition to another).  One cluster more waits for a whole wave: where 15 of 8 fit, 16 of them
+// took 42 us and 15 of 7 take 27.
+struct ClusterCounts {
+    int of[MOST_PARTS + 1] = {0, static_cast<int>(SMS)};
+};
+
+// Asks the device, for sizes up to 8 (portable) and for 16 where `most` allows it.  Once for a device and kernel: the answers take a tenth of a millisecond.
+template <class... Parameters>
+ClusterCounts cluster_counts(void (*kernel)(Parameters...), unsigned threads, std::size_t shared_bytes, int most) {
+    ClusterCounts counts;
+    for (int parts = 2; parts <= most; parts += parts < 8 ? 1 : 8) {
+        cudaLaunchAttribute attribute{};
+        attribute.id = cudaLaunchAttributeClusterDimension;
+        attribute.val.clusterDim.x = static_cast<unsigned>(parts);
+        attribute.val.clusterDim.y = 1;
+        attribute.val.clusterDim.z = 1;
+        cudaLaunchConfig_t config{};
+        config.gridDim = dim3(static_cast<unsigned>(parts));
+        config.blockDim = dim3(threads);
+        config.dynamicSmemBytes = shared_bytes;
+        config.attrs = &attribute;
+        config.numAttrs = 1;
+        if (cudaOccupancyMaxActiveClusters(&counts.of[parts], kernel, &config) != cudaSuccess) {
+            (void)cudaGetLastError();
+            counts.of[parts] = 0;
+        }
+    }
+    return counts;
+}
 
 // What a cluster costs beside its loops in the gradients' kernels: launch, two cluster barriers, the reads.  (Backward of 4064 x 3 rows over 3 x 3821 ragged keys, 180
 // whole loops for 148 SMs: 233 us whole, 144 in parts.)
 constexpr double CLUSTER_US = 4.3;
 
-// Parts that a loop of `tiles` tiles of `tile_us` microseconds is cut into when `ctas` whole loops would run: the cluster size (up to `most`: 8 is portable, 16 has
-// to be allowed) of the shortest time, in as many waves as its clusters need.
-inline int loop_parts(long long ctas, long long tiles, double tile_us, int most) {
+// Parts that a loop of `tiles` tiles of `tile_us` microseconds is cut into when `ctas` whole loops would run: the cluster size of the shortest time, in as many waves
+// as its clusters need.
+inline int loop_parts(long long ctas, long long tiles, double tile_us, const ClusterCounts& counts) {
     int best = 1;
     double best_us = 0.0;
-    for (int parts = 1; parts <= most && parts <= tiles; ++parts) {
-        if (ACTIVE_CLUSTERS[parts] == 0) {
+    for (int parts = 1; parts <= MOST_PARTS && parts <= tiles; ++parts) {
+        if (counts.of[parts] == 0) {
             continue;
         }
-        const long long waves = (ctas + ACTIVE_CLUSTERS[parts] - 1) / ACTIVE_CLUSTERS[parts];
+        const long long waves = (ctas + counts.of[parts] - 1) / counts.of[parts];
         const double us = static_cast<double>(waves) * (static_cast<double>((tiles + parts - 1) / parts) * tile_us + (parts > 1 ? CLUSTER_US : 0.0));
         if (parts == 1 || us < best_us) {
             best = parts;

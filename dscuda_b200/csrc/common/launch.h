@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 
 #include <cstddef>
+#include <mutex>
 #include <utility>
 
 namespace dscuda {
@@ -47,5 +48,27 @@ template <class... Parameters, class... Arguments>
 void launch_chained(void (*kernel)(Parameters...), dim3 grid, dim3 block, std::size_t shared_bytes, cudaStream_t stream, Arguments&&... arguments) {
     launch_chained_clusters(kernel, grid, 1, block, shared_bytes, stream, std::forward<Arguments>(arguments)...);
 }
+
+// What is found out once for each device (the current one), by whichever host thread comes first; on devices behind the table each time.
+template <class Value>
+class PerDevice {
+public:
+    template <class Make>
+    const Value& get(Make&& make) {
+        int device = 0;
+        CUDA_CHECK(cudaGetDevice(&device));
+        if (device >= DEVICES) {
+            thread_local Value value;
+            return value = make();
+        }
+        std::call_once(made_[device], [&] { values_[device] = make(); });
+        return values_[device];
+    }
+
+private:
+    static constexpr int DEVICES = 16;
+    std::once_flag made_[DEVICES];
+    Value values_[DEVICES];
+};
 
 }  // namespace dscuda
