@@ -9,8 +9,8 @@
 //   1. cross_query_kernel: a CTA keeps 128 rows (Q, dO) and goes over the keys in tiles of 128: S = Q K^T, dP = dO V^T, dQ += dS K.  It forms delta from the
 //      O rows first, and leaves lse * log2(e) and delta in row order for the next kernel.  With few keys the rounding of O in delta would be the largest error
 //      of dS (2 keys: 0.4 % of dQ and dK, against 0.17 % of the last rounding); where one tile holds all keys, delta = sum_k P dP is formed
-//      from the tile itself.  One key has no gradient at all (its weight is 1 whatever the score): dS is set to zero on both sides, where dP - delta would
-//      leave what two orders of the same sum differ by.
+//      from the tile itself.  One key has no gradient at all (its weight is 1 whatever the score), where P (dP - delta) would leave what two
+//      orders of the same sum differ by: dQ leaves as zeros (a step inside the loop cost 1-3 % here), and the key side sets dS to zero.
 //   2. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
 //      key (two, half the rows each), P^T and dS^T back into tensor memory as bf16 A operands, dV += P^T dO, dK += dS^T Q.  Tensor memory: dV 128, dK
 //      128, two pairs of 64-column scores, so the scores of the next tile are computed while the softmax works on this one.
@@ -735,8 +735,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                 prob[n] = exp2_approx(fmaf(__uint_as_float(sb[n]), p.scale_log2, -lse2)) * p.scale;
             }
             if (j + 1 == tile_count) {
-                // (a single key's weight is 1 whatever the score: none counts here)
-                const int present = length == 1 ? 0 : left - j * KEYS - half * 64;
+                const int present = left - j * KEYS - half * 64;
 #pragma unroll
                 for (int n = 0; n < 64; ++n) {
                     prob[n] = n < present ? prob[n] : 0.0F;
@@ -798,7 +797,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                         tmem_ld_x32(tmem_base + lane_base + TMEM_DQ + half * 64 + c * 32, values);
                         tmem_wait_ld();
                     }
-                    stage_bf16x32(smem + half * BIG_CHUNK, r, c, values, tile_count > 0);
+                    stage_bf16x32(smem + half * BIG_CHUNK, r, c, values, length > 1);
                 }
                 fence_proxy_async_smem();
                 mbar_arrive(smem_u32(&bars->staged));
@@ -829,7 +828,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_kernel(const __grid_co
                 if (row < row_end) {
                     reinterpret_cast<uint2*>(p.dq_out + ((static_cast<size_t>(entry) * p.tokens + token0 + row / p.group) * p.kv_heads * p.group + kv_head * p.group +
                                                          row % p.group) * HEAD)[lane] =
-                        make_uint2(pack_bf16x2(sums[k].x, sums[k].y), pack_bf16x2(sums[k].z, sums[k].w));
+                        length > 1 ? make_uint2(pack_bf16x2(sums[k].x, sums[k].y), pack_bf16x2(sums[k].z, sums[k].w)) : make_uint2(0, 0);
                 }
             }
         }

@@ -395,8 +395,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_short_kernel(const __g
                     prob[k] = exp2_approx(fmaf(__uint_as_float(sb[k]), p.scale_log2, -lse2)) * p.scale;
                 }
                 if (j + 1 == tile_count) {
-                    // (a single key's weight is 1 whatever the score: none counts here)
-                    const int present = at.length == 1 ? 0 : at.length - j * KEYS - half * 64;
+                    const int present = at.length - j * KEYS - half * 64;
 #pragma unroll
                     for (int k = 0; k < 64; ++k) {
                         prob[k] = k < present ? prob[k] : 0.0F;
@@ -453,7 +452,7 @@ __global__ void __launch_bounds__(THREADS, 1) cross_query_short_kernel(const __g
                 uint32_t values[32];
                 tmem_ld_x32(tmem_base + lane_base + TMEM_DQ + half * 64 + c * 32, values);
                 tmem_wait_ld();
-                stage_bf16x32(smem + place + half * BIG_CHUNK, r, c, values, true);
+                stage_bf16x32(smem + place + half * BIG_CHUNK, r, c, values, at.length > 1);     // (one key: its weight is 1 whatever the score)
             }
             tc_fence_before_sync();
             fence_proxy_async_smem();
