@@ -98,7 +98,7 @@ __global__ void __launch_bounds__(THREADS) flash_cache_append_kernel(const __gri
     sm100::grid_dependency_wait();
     const long long start = p.starts != nullptr ? p.starts[b] : 0;
     const long long count = p.counts != nullptr ? min(max(p.counts[b], 0), p.tokens) : p.tokens;
-    if (start < 0 && threadIdx.x == 0) {
+    if (start < 0 && count > 0 && threadIdx.x == 0) {
         atomicExch(&flash_cache_status, sm100::STATUS_BAD_INDEX);       // its tokens in front of position 0 are left out
     }
     const long long logical = max(start, 0LL) / p.page + blockIdx.x;
