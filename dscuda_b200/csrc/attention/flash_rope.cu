@@ -5,10 +5,10 @@
 //     out[i + W/2] = x[i] * sin + x[i + W/2] * cos
 // (sin changes sign for `inverse`, which is the transpose and so the gradient).
 //
-// Angles.  position * f_i / (2 pi) is formed in double precision and reduced to the nearest whole turn there.  Its fp32 part goes through sincospif, what that
-// leaves over (up to 2^-25 of half a turn) is turned on to first order: the error is that of fp32 sines at any position, and a bf16 result rounds as the exact one
-// but for about one in 2^15.  The products and sums are separate fp32 operations, rounded
-// once to bf16.
+// Angles.  position * f_i / (2 pi) is formed in double precision and reduced to the nearest whole turn there; sine and cosine are taken in double precision
+// and rounded to fp32, the products and sums are separate fp32 operations, rounded once to bf16.  So a result has the bits that these steps have anywhere else, and
+// codes made from it (the 8-bit cache) are the same; with fp32 sines one result in 2^15 rounded to its neighbour.  That costs nothing at 16384 rows of
+// 32 + 8 heads (55.1 us) and 2 % where a row has 8 heads (16.3 us, with fp32 sines 16.0).
 //
 // Bound: HBM, every value is read and written once.  A warp takes a row: its lanes compute the row's W/2 sines and cosines once (two or
 // one each) and exchange them through shared memory; then W/16 lanes cover a head, a lane with 16 bytes of either half, and the warp goes over
@@ -86,12 +86,9 @@ __global__ void __launch_bounds__(ROPE_THREADS, 3) flash_rope_kernel(const __gri
 #pragma unroll
         for (int k = 0; k < OWN; ++k) {
             const double whole = p.positions[axis[k] * p.rows + row] * frequency[k];
-            const double half_turns = 2.0 * (whole - rint(whole));
-            const float high = static_cast<float>(half_turns);
-            const float rest = static_cast<float>(half_turns - high) * 3.14159265F;
-            float s, c;
-            sincospif(high, &s, &c);
-            turns[warp][lane + 32 * k] = make_float2(fmaf(-s, rest, c), fmaf(c, rest, s) * p.sign);
+            double s, c;
+            sincospi(2.0 * (whole - rint(whole)), &s, &c);
+            turns[warp][lane + 32 * k] = make_float2(static_cast<float>(c), static_cast<float>(s) * p.sign);
         }
         __syncwarp();
         float2 turn[8];
