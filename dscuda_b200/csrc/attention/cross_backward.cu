@@ -7,9 +7,9 @@
 //
 // One call launches:
 //   1. cross_query_kernel: a CTA keeps 128 rows (Q, dO) and goes over the keys in tiles of 128: S = Q K^T, dP = dO V^T, dQ += dS K.  It forms delta from the
-//      O rows first, and leaves lse * log2(e) and delta in row order for the next kernel.  With few keys the rounding of O in delta would be the largest error
-//      of dS (2 keys: 0.4 % of dQ and dK, against 0.17 % of the last rounding); where one tile holds all keys, delta = sum_k P dP is formed
-//      from the tile itself.  One key has no gradient at all (its weight is 1 whatever the score), where P (dP - delta) would leave what two
+//      O rows first, and leaves lse * log2(e) and delta in row order for the next kernel.  Where a softmax sits on few keys, the rounding of O in delta is the largest error
+//      of dS (2 keys: 0.4 % of dQ and dK, against 0.17 % of the last rounding).  Up to 128 keys, one tile, delta = sum_k P dP is formed from the tile itself and free
+//      of it; longer entries keep that error, as two passes over the keys would be the price.  One key has no gradient at all (its weight is 1 whatever the score), where P (dP - delta) would leave what two
 //      orders of the same sum differ by: dQ leaves as zeros (a step inside the loop cost 1-3 % here), and the key side sets dS to zero.
 //   2. cross_key_kernel: a CTA keeps 128 keys (K, V) and goes over the rows in tiles of at most 64: S^T = K Q^T, dP^T = V dO^T, one thread to a
 //      key (two, half the rows each), P^T and dS^T back into tensor memory as bf16 A operands, dV += P^T dO, dK += dS^T Q.  Tensor memory: dV 128, dK

@@ -13,7 +13,8 @@
 // chunk's successor is on its way as soon as the products that read it are done.
 //
 // Warps 0-3 are the softmax, warp 4 issues the MMAs, warp 5 the loads; warps 6 and 7 clear the value rows behind an entry's length (a weight of zero
-// does not keep their NaN out of P V).  The second warpgroup hands registers to the softmax, which holds a row of scores.
+// does not keep their NaN out of P V).  The second warpgroup hands registers to the softmax, which holds a row of scores.  Two CTAs to an SM leave the compiler 128
+// registers at launch, and it spills 132 bytes of a thread's state around the scores.
 //
 // Small problems: where the tiles would leave SMs idle the loop over the keys is cut into parts for the CTAs of a cluster, which join their fp32 sums
 // through distributed shared memory (loop_parts.cuh).

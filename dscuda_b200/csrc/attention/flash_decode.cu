@@ -11,11 +11,13 @@
 // far below the tensor core's ratio, so the products run on mma.sync (m16n8k16, fp32 sums): 16 rows fit its tile, its operands
 // come from registers where the codes are widened on the way, and at the copy rate it is a third busy.  tcgen05 wants the
 // widened tile written back to shared memory, 192 KB of traffic a tile: measured over 8 sequences of 20000-40000 positions it took 140 us for 32
-// rows (this form 116) and 154 for 64 (213: the cache is read twice), over 32 sequences of 500-4000 114 us for 64 rows (96).  Steps of single
-// tokens and short drafts are what this is for, so the one form serves all.
+// rows (this form 116 at the time, 118-125 from box to box now) and 154 for 64 (213: the cache is read twice), over 32 sequences of 500-4000 114 us for
+// 64 rows (96).  That was with f16 operands; the 8-bit kinds, which could read the codes as they lie but want the rows as several 8-bit terms, were
+// not tried.  Steps of single tokens and short drafts are what this is for, so the one form serves all.
 //
-// Measured (64 query heads on 8): 32 sequences of 1000-8000 tokens 46.5 us (floor 38.3), 4 drafted tokens at 20000-40000 120 us (floor
-// 72.7; bound by the issue of widening and softmax beside the copies), one sequence of 100 tokens 4.0 us (one launch; 5.4 in parts).
+// Measured: 32 sequences of 1-8192 tokens, 32 query heads on 8, 46.5-47.5 us (floor 38.3); 4 drafted tokens at 20000-40000, 64 on 8, 118-125 us (floor 72.7);
+// 8 items of 128 keys 4.4 us (one launch; 6.5 in parts).  With 32 rows no unit is the bound (DRAM 47 %, tensor 46 %, issue 39 %): the forms of 32 rows take 255
+// registers and spill 28-48 bytes, so that two CTAs, eight warps, are all an SM holds, and these do not cover the latency of a step.
 //
 // Operands.  Codes become f16 (exact for both types: int8 through 1024 + u - 1152, e4m3 by conversion) and so does Q, each row
 // multiplied by a power of two that brings its largest element to 2^13..2^14; P is rounded to f16 (half a step is 2^-11 of it), relative to the
@@ -31,8 +33,9 @@
 //
 // Work split: tiles of 4 warps x 32 (16) keys of all (sequence, head, row block) items laid end to end and cut into equal ranges, one
 // per CTA.  A warp streams its own keys through its own ring (cp.async, no barriers between warps); the four merge at the end of an
-// item.  Short items stay whole (stays_whole).  Otherwise an item that one CTA sees whole is written at once, parts go to the workspace, and the CTA with an item's first tile leaves a
-// note of who holds them; flash_decode_combine_kernel joins them.  Where all items are short each stays with a CTA of its own (stays_whole).  No atomics: results do not depend on the order in which CTAs run.
+// item.  An item that one CTA sees whole is written at once, parts go to the workspace, and the CTA with an item's first tile leaves a
+// note of who holds them; flash_decode_combine_kernel joins them.  Where no item can be long each stays with a CTA of its own (stays_whole).  No atomics: results do
+// not depend on the order in which CTAs run.
 #include "flash_attention.h"
 #include "cuda_common.h"
 #include "attention_internal.h"
@@ -898,9 +901,11 @@ __global__ void __launch_bounds__(THREADS) flash_decode_combine_kernel(const __g
 }
 
 // Whether every item stays whole, with a CTA of its own and no second kernel: up to so many keys the time of the longest item is below that of the parts and
-// their joining.  us, parts and whole, lengths down to a third or less: 32 items of up to 400 keys 9.4 and 6.8, 640 8.7 and 8.0; 64 of 900 10.3 and 10.4; 128 of 512
+// their joining.  us, parts and whole, lengths down to a third or less: 8 items of up to 128 keys 6.5 and 4.4, 384 7.3 and 6.3, 512 7.3 and 7.1, 700 7.4 and 8.1 (16 rows: 384 8.8 and
+// 8.1, 512 8.7 and 9.5); 32 items of up to 400 keys 9.4 and 6.8, 640 8.7 and 8.0; 64 of 900 10.3 and 10.4; 128 of 512
 // 10.8 and 8.2, 768 12.5 and 10.0, bf16 states of 1000 13.0 and 13.6; 200 of 1000 15.0 and 14.0, 1500 16.6 and 16.4, 2000 18.3 and 21.4; 512 of 512 17.8 and 15.7, 800
-// 19.6 and 19.3, 1200 25.6 and 27.1.  (The longest is what the caller's table or tensor holds; lengths are not known here.)
+// 19.6 and 19.3, 1200 25.6 and 27.1.  More items bear longer ones, as the parts' CTAs have several each to go over; from more items than CTAs run at once on, whole items
+// need a second wave.  The longest is what the caller's table or tensor holds: lengths are not known here, so a wide table over short sequences takes the parts.
 bool stays_whole(long long items, int keys_most, int at_once) {
     return keys_most <= (items > at_once ? 768 : items >= 200 ? 1280 : items >= 96 ? 896 : items >= 32 ? 704 : 384);
 }

@@ -38,7 +38,7 @@ def cache_append(key_cache, value_cache, key_scale, value_scale, key, value, blo
     (0 / all T tokens).  Token t of sequence b lands at position start_positions[b] + t.
     A page's scale covers what the page holds: where new values need a larger one, the page's older codes are rounded again.  What
     a sequence held at and behind its first new position is given up.  A page must not be written twice in one call (two sequences that share it have
-    to part before).  Positions and page numbers outside the cache are skipped and raise status 3 (`device_status`)."""
+    to part before).  Positions and page numbers outside the cache are skipped and raise status 3 (`device_status`); an entry without tokens has none."""
     extension().flash_cache_append(key_cache, value_cache, key_scale, value_scale, key, value, block_table, start_positions, token_counts)
 
 
@@ -52,7 +52,8 @@ def decode(query, key_cache, value_cache, key_scale, value_scale, block_table, c
     """Attention of the newest T tokens over the 8-bit cache (`dscuda_flash_decode`), T at most 64.
     query [B, T, Hq, 128]; cache and block_table as for `cache_append`; cache_lengths [B] int32, the new tokens included: token t sees the
     first cache_lengths[b] - T + 1 + t positions -> (output [B, T, Hq, 128], lse [B, Hq, T] fp32).  A token that sees none gets zeros and -inf.
-    Page numbers outside the cache are read as page 0 and raise status 3."""
+    Page numbers outside the cache are read as page 0 and raise status 3.  The width of block_table (what it can hold, not the lengths) picks how the work is cut: trimmed to
+    the longest sequence it is faster for short ones, and another width may change the last bits."""
     return extension().flash_decode(query, key_cache, value_cache, key_scale, value_scale, block_table, cache_lengths, scale, workspace, output, lse)
 
 
@@ -66,7 +67,7 @@ def cross_forward(query, key, value, scale, key_lengths=None, workspace=None, ou
     """Attention to an encoder's states (`dscuda_flash_cross_forward`): no causal mask, Hq / Hkv at most 64.
     query [B, Tq, Hq, 128], key, value [B, Tk, Hkv, 128], key_lengths [B] int32 or None (all Tk): every query sees the first
     key_lengths[b] keys -> (output [B, Tq, Hq, 128], lse [B, Hq, Tq] fp32).  An entry without keys gets zeros and -inf; what lies behind
-    a length is not used, NaN included."""
+    a length is not used, NaN included.  Sizes pick how the work is cut: another padding Tk may change the last bits."""
     return extension().flash_cross_forward(query, key, value, scale, key_lengths, workspace, output, lse)
 
 
@@ -78,5 +79,5 @@ def cross_backward_workspace(batch, query_length, key_length, query_heads, key_v
 
 def cross_backward(dout, output, lse, query, key, value, scale, key_lengths=None, workspace=None, grads=None):
     """Gradients of `cross_forward` (`dscuda_flash_cross_backward`) from its output and lse -> (dquery, dkey, dvalue).
-    Keys behind an entry's length get zeros.  The same bits from call to call."""
+    Keys behind an entry's length get zeros, as do the queries and the key of an entry with a single key.  The same bits from call to call."""
     return extension().flash_cross_backward(dout, output, lse, query, key, value, scale, key_lengths, workspace, grads)

@@ -78,7 +78,7 @@ constexpr int FLASH_DECODE_MAX_TOKENS = 64;
 // the new one.  code = round-half-even(x * (1 / scale)).  NaN becomes 0, an infinity the largest code; neither counts for the scale.
 // What a page held at and behind the first new position is given up, whether it is written over or not (its codes do not follow the scale).  A
 // page must not be written twice in one call, for two sequences or for one.  A position or page number outside the cache is not written
-// and sets the device status to 3.
+// and sets the device status to 3 (an entry without tokens has no position, whatever its start).
 void flash_cache_append_cuda(
     void* key_cache,
     void* value_cache,
@@ -109,6 +109,9 @@ std::size_t flash_decode_workspace_bytes(int batch_size, int tokens, int query_h
 // none gets zeros and -inf.  Lengths are read as at least 0 and at most pages_per_sequence * page_size; a page number
 // outside [0, cache_blocks) is read as page 0 and sets the device status to 3.  Calls that may run at the same time need
 // workspaces of their own.
+// How the work is cut depends on what the table can hold (batch, heads and pages_per_sequence * page_size): where that is short (384 to 1280 positions) a sequence stays
+// with one CTA to a head and row block and there is one launch, otherwise its parts are joined by a second kernel.  So a table trimmed to the longest sequence
+// is the faster one for short sequences, and the same sequence may get other last bits in a table of another width; the same arguments get the same bits.
 void flash_decode_cuda(
     __nv_bfloat16* output,
     float* logsumexp,
@@ -136,7 +139,8 @@ void flash_decode_cuda(
 // Cross attention: every query sees the first key_lengths[b] of its entry's Tk keys (all when key_lengths is null; lengths are read as
 // at least 0 and at most Tk).  query, output [B,Tq,Hq,128], key, value [B,Tk,Hkv,128], logsumexp [B,Hq,Tq].  An entry without keys gets
 // zeros and -inf.  What lies behind an entry's length is never used, NaN included.  Calls that may run at the same time need
-// workspaces of their own; the size may be 0 (then workspace may be null).
+// workspaces of their own; the size may be 0 (then workspace may be null).  How the work is cut depends on the sizes, Tk among them, not on the lengths: another
+// padding may give other last bits, the same arguments give the same.
 std::size_t flash_cross_forward_workspace_bytes(int batch_size, int query_length, int key_length, int query_heads, int key_value_heads);
 
 void flash_cross_forward_cuda(
@@ -157,8 +161,9 @@ void flash_cross_forward_cuda(
     float scale,
     cudaStream_t stream = nullptr);
 
-// Its gradients, BF16 in the shapes of query, key and value, overwritten; those of keys behind an entry's length are zero.  No atomics:
-// two calls on the same inputs return the same bits.
+// Its gradients, BF16 in the shapes of query, key and value, overwritten; those of keys behind an entry's length are zero, and so are those of the queries and the
+// key of an entry with a single key, whose weight is 1 whatever the score.  In entries of more than 128 keys the rounding of `output` reaches the gradients
+// (through delta: 0.4 % of them where a softmax sits on two keys).  No atomics: two calls on the same inputs return the same bits.
 std::size_t flash_cross_backward_workspace_bytes(int batch_size, int query_length, int key_length, int query_heads, int key_value_heads);
 
 void flash_cross_backward_cuda(
