@@ -550,25 +550,7 @@ DSCUDA_FUNCTION(prefill_backward) {
     });
 }
 
-// query, key, value, scale -> output, lse
-DSCUDA_FUNCTION(flash_forward) {
-    return guarded([&] {
-        expect_arguments(count, 4);
-        const Tensor &query = tensor(args[0], 4), &key = tensor(args[1]), &value = tensor(args[2]);
-        const float scale = number(args[3]);
-        const int b = extent(query, 0), t = extent(query, 1), hq = extent(query, 2), d = extent(query, 3), hkv = extent(key, 2);
-        Tensor output = new_like(query);
-        Tensor lse = new_tensor({b, hq, t}, query, at::kFloat);
-        void* stream = current_stream();
-        checked(dscuda_flash_last_error, [&] {
-            return dscuda_flash_forward(pointer(output), static_cast<float*>(pointer(lse)), pointer(query), pointer(key), pointer(value), b, t, hq, hkv, d,
-                                        scale, stream);
-        });
-        return tuple(output, lse);
-    });
-}
-
-// ---- grouped-query operators around flash_forward (dscuda_b200/flash.py) ----------------------
+// ---- grouped-query operators (dscuda_b200/flash.py) ----------------------
 // Inputs of these calls are checked for device, type and shape as well; work goes to the inputs' device and its current stream.
 void expect_input(const Tensor& t, const Tensor& like, at::ScalarType type, at::IntArrayRef sizes, const char* what) {
     if (t.device() != like.device()) {
@@ -632,6 +614,34 @@ struct OnDevice {
     void* stream;
     explicit OnDevice(const Tensor& t) : guard(t.device()), stream(c10::cuda::getCurrentCUDAStream(t.device().index()).stream()) {}
 };
+
+// query, key, value, scale -> output, lse
+DSCUDA_FUNCTION(flash_forward) {
+    return guarded([&] {
+        expect_arguments(count, 4);
+        const Tensor &query = tensor(args[0], 4), &key = tensor(args[1], 4), &value = tensor(args[2]);
+        const float scale = number(args[3]);
+        const int b = extent(query, 0), t = extent(query, 1), hq = extent(query, 2), d = extent(query, 3), hkv = extent(key, 2);
+        expect_input(query, query, at::kBFloat16, query.sizes(), "the query");
+        // (one entry may have more keys and values behind the tokens: they are not read)
+        const Tensor* states[2] = {&key, &value};
+        const char* names[2] = {"the key", "the value"};
+        for (int i = 0; i < 2; ++i) {
+            expect_input(*states[i], query, at::kBFloat16, states[i]->sizes(), names[i]);
+            if (states[i]->numel() < query.size(0) * query.size(1) * key.size(2) * query.size(3)) {
+                fail(PyExc_ValueError, std::string(names[i]) + " has fewer elements than the query's tokens need");
+            }
+        }
+        Tensor output = new_like(query);
+        Tensor lse = new_tensor({b, hq, t}, query, at::kFloat);
+        const OnDevice on(query);
+        checked(dscuda_flash_last_error, [&] {
+            return dscuda_flash_forward(pointer(output), static_cast<float*>(pointer(lse)), pointer(query), pointer(key), pointer(value), b, t, hq, hkv, d,
+                                        scale, on.stream);
+        });
+        return tuple(output, lse);
+    });
+}
 
 bool truth(PyObject* object) {
     const int value = PyObject_IsTrue(object);
