@@ -11,7 +11,7 @@
 // far below the tensor core's ratio, so the products run on mma.sync (m16n8k16, fp32 sums): 16 rows fit its tile, its operands
 // come from registers where the codes are widened on the way, and at the copy rate it is a third busy.  tcgen05 wants the
 // widened tile written back to shared memory, 192 KB of traffic a tile: measured over 8 sequences of 20000-40000 positions it took 140 us for 32
-// rows (this form 116 at the time, 118-125 from box to box now) and 154 for 64 (213: the cache is read twice), over 32 sequences of 500-4000 114 us for
+// rows (this form 116 at the time, 118-125 by now) and 154 for 64 (213: the cache is read twice), over 32 sequences of 500-4000 114 us for
 // 64 rows (96).  That was with f16 operands; the 8-bit kinds, which could read the codes as they lie but want the rows as several 8-bit terms, were
 // not tried.  Steps of single tokens and short drafts are what this is for, so the one form serves all.
 //
