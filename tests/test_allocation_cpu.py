@@ -24,17 +24,17 @@ def fake(*shape, dtype=torch.bfloat16):
 
 
 CALLS = {
-    "mla_forward": (mla.mla_forward, fake(1, 3, 2, 512), fake(1, 3, 2, 64), fake(1, 3, 512), fake(1, 3, 64), 0.1),
-    "prefill_forward": (mla.prefill_forward, fake(1, 5, 2, 128), fake(1, 5, 2, 64), fake(1, 5, 2, 128), fake(1, 5, 1, 64), fake(1, 5, 2, 128), 0.1),
-    "absorb_query": (mla.absorb_query, fake(4, 2, 128), fake(256, 512)),
-    "flash_forward": (mla.flash_forward, fake(1, 64, 4, 128), fake(1, 64, 2, 128), fake(1, 64, 2, 128), 0.1),
-    "rope": (flash.rope, fake(4, 2, 128), None, fake(1, 4, dtype=torch.int32), [64]),
-    "cross_forward": (flash.cross_forward, fake(1, 50, 4, 128), fake(1, 60, 2, 128), fake(1, 60, 2, 128), 0.1),
+    "mla_forward": lambda: (mla.mla_forward, fake(1, 3, 2, 512), fake(1, 3, 2, 64), fake(1, 3, 512), fake(1, 3, 64), 0.1),
+    "prefill_forward": lambda: (mla.prefill_forward, fake(1, 5, 2, 128), fake(1, 5, 2, 64), fake(1, 5, 2, 128), fake(1, 5, 1, 64), fake(1, 5, 2, 128), 0.1),
+    "absorb_query": lambda: (mla.absorb_query, fake(4, 2, 128), fake(256, 512)),
+    "flash_forward": lambda: (mla.flash_forward, fake(1, 64, 4, 128), fake(1, 64, 2, 128), fake(1, 64, 2, 128), 0.1),
+    "rope": lambda: (flash.rope, fake(4, 2, 128), None, fake(1, 4, dtype=torch.int32), [64]),
+    "cross_forward": lambda: (flash.cross_forward, fake(1, 50, 4, 128), fake(1, 60, 2, 128), fake(1, 60, 2, 128), 0.1),
 }
 
 
 @pytest.mark.parametrize("name", CALLS)
 def test_dispatch_modes_see_new_tensors(name):
-    call, *arguments = CALLS[name]
+    call, *arguments = CALLS[name]()
     with pytest.raises(Seen, match="cuda"), Watch():
         call(*arguments)

@@ -14,14 +14,14 @@ def fake(*shape, dtype=torch.bfloat16, device="cuda:0"):
 
 
 def call(query=(2, 70, 8, 128), key=(2, 70, 2, 128), value=(2, 70, 2, 128), **given):
-    return flash.forward(*[given.get(name, fake(*shape)) for name, shape in (("query_", query), ("key_", key), ("value_", value))], 0.1)
+    return flash.forward(*[fake(*shape, **given.get(name, {})) for name, shape in (("query_", query), ("key_", key), ("value_", value))], 0.1)
 
 
 @pytest.mark.parametrize("given,message", [
     (dict(key=(2, 69, 2, 128)), "the key has fewer"), (dict(value=(2, 40, 2, 128)), "the value has fewer"), (dict(value=(2, 70, 1, 128)), "the value has fewer"),
     (dict(key=(1, 70, 2, 128)), "the key has fewer"), (dict(key=(2, 70, 2, 64)), "the key has fewer"),
-    (dict(query_=fake(2, 70, 8, 128, dtype=torch.float16)), "the query has the wrong dtype"), (dict(key_=fake(2, 70, 2, 128, dtype=torch.float32)), "the key has the wrong dtype"),
-    (dict(value_=fake(2, 70, 2, 128, device="cuda:1")), "the value is on another device"), (dict(key=(140, 2, 128)), "4 dimensions"),
+    (dict(query_=dict(dtype=torch.float16)), "the query has the wrong dtype"), (dict(key_=dict(dtype=torch.float32)), "the key has the wrong dtype"),
+    (dict(value_=dict(device="cuda:1")), "the value is on another device"), (dict(key=(140, 2, 128)), "4 dimensions"),
 ])
 def test_refused(given, message):
     with pytest.raises(ValueError, match=message):
